@@ -386,7 +386,7 @@ def _plain_verify(st):
             x = st["ids"][kid_row].long()[:, None]
             testing = walking & (kid < Q) & (found < 0)
             rx = torch.gather(r, 1, x)[:, 0]
-            picked = u[kid_row] * (1 - gone) < rx
+            picked = (rx > 0) & (u[kid_row] * (1 - gone) < rx)
             if st["draft_rows"] is None:
                 ok = picked
                 off = testing & ~ok
@@ -528,7 +528,7 @@ def _exact_drafts(st):
             for i in kids:
                 x = ids[a + i]
                 if d is None:
-                    if u[a + i] * left < float(r[x]):
+                    if 0 < float(r[x]) > u[a + i] * left:
                         path.append(i)
                         moved = True
                         break
