@@ -294,6 +294,90 @@ int tb_embed(const int* ids, int M, const void* emb, int ld_emb, int d, int voca
  * Replaces the greedy branch of LLMEngine._sample (src/tinybatch/engine.py:149-151). */
 int tb_argmax(const float* logits, int ld, int M, int N, int* out, void* stream);
 
+/* --------------------------------------------------- speculative decoding
+ * (no counterpart in the reference, which decodes one token a step)
+ *
+ * A sequence's draft tree: node i is row q_start[s] + i of the flat batch
+ * (i < q_len[s] <= 256), node 0 the root (the last accepted token, whose K/V
+ * the same forward writes), parents[row] < i the parent's node index (-1 for
+ * the root).  Node i's K/V lie at position ctx_len[s] - q_len[s] + i of the
+ * sequence.  Sequences with q_len 0 take part in nothing.  max_q >= every
+ * q_len.  Rows of different sequences do not overlap. */
+
+/* Attention of draft-tree nodes over the paged cache; arguments as
+ * tb_paged_attention_decode, bt_w the columns of a block-table row (bt_ld
+ * its pitch).  Node i sees the positions before the root
+ * (0 .. ctx_len-q_len-1) and the nodes j whose bit (bit j % 64 of word j / 64)
+ * is set in row i of tree_mask [n_rows, mask_ld] uint64, mask_words (1..4)
+ * words used.  A row that sees nothing gets zeros.  Whatever keys and values
+ * a row does not see hold (NaN included) does not reach it.  Rows of out
+ * that belong to no sequence are left as they were.
+ * max_ctx / ctx_total: the longest context and their sum, for choosing how
+ * many thread blocks share a context (hints: any value gives right results;
+ * 0 = bt_w * block_size / n_seqs times that).  No scratch: the blocks that
+ * share a context form a cluster and merge through shared memory.
+ * A sequence whose rows leave the batch, whose q_len exceeds max_q or the
+ * mask, or whose context its block-table row cannot hold, and block ids out
+ * of range set TB_STATUS_BAD_INDEX. */
+int tb_paged_attention_tree(const void* q, int ld_q, void* out, int ld_out, int n_rows,
+                            const void* kv_pool, int num_blocks, int n_q_heads,
+                            int n_kv_heads, int head_dim, int block_size,
+                            const int* block_tables, int bt_ld, int bt_w, const int* q_start,
+                            const int* q_len, const int* ctx_len, int n_seqs,
+                            const void* tree_mask, int mask_ld, int mask_words,
+                            int max_q, int max_ctx, long long ctx_total, void* stream);
+
+/* Verification of the drafts.  ids / parents [n_rows] int32.  Outputs per
+ * sequence: path[s, 0..path_w) the accepted nodes in order, the root first,
+ * -1 after them; n_accepted[s] how many drafts that is (without the root);
+ * next_ids[s] the token that follows the last of them.  A walk that has
+ * filled its path stops there.  q_len 0 gives path -1, n_accepted 0, next -1.
+ * Parents that are no earlier node, ids outside the vocabulary and rows
+ * outside the batch set TB_STATUS_BAD_INDEX; such nodes are never accepted.
+ *
+ * _greedy: the accepted child is the first whose id is target_ids[row of the
+ * node] (the target's argmax there); next is target_ids of the last node.
+ *
+ * Sampled: probs [n_rows, vocab] fp32 (pitch ld_probs), the target's
+ * distribution after each node; uniforms [n_rows] in [0, 1): a draft's own
+ * number decides its test, the root's the final sample.  draft_probs
+ * [n_draft_rows, vocab] fp32 and draft_rows [n_rows]: the distribution a
+ * node's children were drawn from without replacement, -1 where they were
+ * picked outright (both NULL: everywhere).  Rows are finite, non-negative
+ * and sum to one; the accepted tokens and next then follow the target's
+ * distribution.  next is -1 where the last row has no positive entry.  The
+ * formulas stand in csrc/verify.cu. */
+int tb_verify_drafts_greedy(const int* ids, const int* parents, const int* q_start,
+                            const int* q_len, int n_seqs, int n_rows, int max_q,
+                            const int* target_ids, int* n_accepted, int* path, int path_ld,
+                            int path_w, int* next_ids, void* stream);
+int tb_verify_drafts(const int* ids, const int* parents, const int* q_start, const int* q_len,
+                     int n_seqs, int n_rows, int max_q, const float* probs, long long ld_probs,
+                     int vocab, const float* draft_probs, long long ld_draft, int n_draft_rows,
+                     const int* draft_rows, const float* uniforms, int* n_accepted, int* path,
+                     int path_ld, int path_w, int* next_ids, void* stream);
+
+/* Cache moves in every layer of pools_h (a host array of n_layers device
+ * pointers, each a pool [num_blocks, 2, n_kv_heads, block_size, head_dim]
+ * bf16, head_dim a multiple of 8; distinct pools).
+ *
+ * _keep_kv_path: after verification, the K/V of path[s, j] (j = 1 ..
+ * n_accepted[s], strictly increasing nodes) move to node j's place, so the
+ * accepted tokens lie at consecutive positions after the root.  A sequence
+ * with a bad path or block table sets TB_STATUS_BAD_INDEX and moves nothing.
+ * Sequences must not share the blocks that hold their drafts.
+ *
+ * _copy_kv_blocks: pairs [n_pairs, 2] int32 of (source, destination) block
+ * ids.  Copies run in no order, so a pair whose destination is another
+ * pair's source or destination, like one with an id out of range, sets
+ * TB_STATUS_BAD_INDEX and is not made. */
+int tb_keep_kv_path(const void* const* pools_h, int n_layers, int num_blocks, int n_kv_heads,
+                    int block_size, int head_dim, const int* block_tables, int bt_ld, int bt_w,
+                    const int* q_len, const int* ctx_len, const int* path, int path_ld, int path_w,
+                    const int* n_accepted, int n_seqs, void* stream);
+int tb_copy_kv_blocks(const void* const* pools_h, int n_layers, int num_blocks, int n_kv_heads,
+                      int block_size, int head_dim, const int* pairs, int n_pairs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,230 @@
+"""Speculative decoding without a GPU: argument errors of the C entry points,
+draft-tree masks and step metadata, block tables of forks and rejected drafts,
+and the 64-bit restatement the GPU tests compare against."""
+from __future__ import annotations
+
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import speculative_ref as R
+from tinybatch_b200 import _native as N
+from tinybatch_b200 import ops
+from tinybatch_b200.block_manager import BlockManager, OutOfBlocks
+from tinybatch_b200.kv_cache import PagedKVCache
+from tinybatch_b200.runtime import StepMeta, tree_masks
+
+P = 256     # stands for an aligned pointer that is never followed
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not N.lib_path().exists():
+        from tinybatch_b200 import build
+        build.build()
+    return N.load()
+
+
+def attention(lib, **kw):
+    a = dict(q=P, ld_q=256, out=P, ld_out=256, rows=4, pool=P, blocks=8, hq=4, hkv=2, hd=64, bs=16, bt=P,
+             bt_ld=4, bt_w=4, q_start=P, q_len=P, ctx=P, n=1, mask=P, mask_ld=1, words=1, max_q=4, max_ctx=0,
+             total=0, stream=None)
+    a.update(kw)
+    return lib.tb_paged_attention_tree(*a.values())
+
+
+@pytest.mark.parametrize("change,needle", [
+    (dict(hq=5), "heads"), (dict(hkv=0), "heads"), (dict(hq=516, ld_q=33024, ld_out=33024), "GQA group"),
+    (dict(hd=96), "head_dim"), (dict(bs=0), "block_size"), (dict(blocks=0), "num_blocks"),
+    (dict(bt_w=0), "block table"), (dict(bt_ld=-1), "block table"), (dict(ld_q=252), "ld_q"),
+    (dict(ld_out=128), "ld_out"), (dict(words=0), "words"), (dict(words=5, mask_ld=5), "words"),
+    (dict(words=2), "words"), (dict(max_q=65), "max_q"), (dict(max_q=-1), "max_q"), (dict(n=-1), "n_seqs"),
+    (dict(n=70000), "65535"), (dict(q=None), "null pointer"), (dict(mask=None), "null pointer"),
+    (dict(ctx=None), "null pointer"), (dict(pool=P + 8), "aligned"), (dict(out=P + 2), "aligned")])
+def test_attention_argument_errors(lib, change, needle):
+    assert attention(lib, **change) == 1
+    assert needle in lib.tb_last_error().decode()
+
+
+@pytest.mark.parametrize("change", [dict(n=0), dict(max_q=0), dict(rows=0, max_q=0)])
+def test_attention_of_nothing_launches_nothing(lib, change):
+    assert attention(lib, q=None, **change) == 0
+
+
+def verify(lib, **kw):
+    a = dict(ids=P, parents=P, q_start=P, q_len=P, n=1, rows=4, max_q=4, probs=P, ld=100, vocab=100, draft=None,
+             ld_d=0, n_d=0, d_rows=None, u=P, took=P, path=P, path_ld=4, path_w=4, nxt=P, stream=None)
+    a.update(kw)
+    return lib.tb_verify_drafts(*a.values())
+
+
+@pytest.mark.parametrize("change,needle", [
+    (dict(n=-1), "n_seqs"), (dict(rows=-1), "n_rows"), (dict(path_w=0), "path"), (dict(path_ld=3), "path"),
+    (dict(max_q=257), "256 nodes"), (dict(ids=None), "null pointer"), (dict(nxt=None), "null pointer"),
+    (dict(vocab=0), "vocab"), (dict(ld=99), "vocab"), (dict(probs=None), "probs"), (dict(u=None), "uniforms"),
+    (dict(draft=P), "go together"), (dict(d_rows=P), "go together"),
+    (dict(draft=P, d_rows=P, ld_d=99, n_d=1), "draft_probs"), (dict(draft=P, d_rows=P, ld_d=100, n_d=-1), "draft")])
+def test_verify_argument_errors(lib, change, needle):
+    assert verify(lib, **change) == 1
+    assert needle in lib.tb_last_error().decode()
+
+
+def test_verify_of_nothing_launches_nothing(lib):
+    assert verify(lib, n=0, ids=None) == 0
+    assert lib.tb_verify_drafts_greedy(None, None, None, None, 0, 0, 0, None, None, None, 1, 1, None, None) == 0
+    assert lib.tb_verify_drafts_greedy(P, P, P, P, 1, 4, 4, None, P, P, 4, 4, P, None) == 1
+
+
+def pools_h(*ptrs):
+    import ctypes
+    return (ctypes.c_void_p * len(ptrs))(*ptrs)
+
+
+def test_cache_move_argument_errors(lib):
+    def copy(pools, layers=1, blocks=4, hkv=2, bs=16, hd=64, pairs=P, n=1):
+        return lib.tb_copy_kv_blocks(pools, layers, blocks, hkv, bs, hd, pairs, n, None)
+
+    def keep(pools, layers=1, hd=64, bt_ld=4, bt_w=4, path_ld=4, path_w=4, path=P, n=1):
+        return lib.tb_keep_kv_path(pools, layers, 4, 2, 16, hd, P, bt_ld, bt_w, P, P, path, path_ld, path_w, P, n,
+                                   None)
+
+    one = pools_h(P)
+    for rc, needle in [(copy(one, blocks=0), "pool shape"), (copy(one, hd=12), "head_dim"),
+                       (copy(None), "pools_h"), (copy(pools_h(P + 8)), "aligned"), (copy(pools_h(None)), "aligned"),
+                       (copy(one, n=-1), "n_pairs"), (copy(one, pairs=None), "pairs"),
+                       (copy(one, pairs=P + 4), "pairs")]:
+        assert rc == 1
+    for change, needle in [(dict(hd=12), "head_dim"), (dict(bt_w=0), "bt_ld"), (dict(path_w=0), "path"),
+                           (dict(path_ld=3), "path"), (dict(path=None), "null pointer"), (dict(n=-1), "n_seqs")]:
+        assert keep(one, **change) == 1
+        assert needle in lib.tb_last_error().decode()
+    assert copy(one, n=0) == 0 and copy(None, layers=0) == 0 and keep(one, n=0) == 0
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.KVPools(torch.zeros(1, 4, 2, 1, 16, 64, dtype=torch.bfloat16))
+    t = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.verify_drafts_greedy(t, t, t, t, t, t, t[None], t)
+
+
+def test_copy_blocks_checks_its_pairs_on_the_host():
+    cache = PagedKVCache(1, 4, 16, 1, 64, device="cpu")
+    cache.copy_blocks([])
+    with pytest.raises(IndexError):
+        cache.copy_blocks([(0, 4)])
+    with pytest.raises(IndexError):
+        cache.copy_blocks([(-1, 2)])
+    with pytest.raises(ValueError):
+        cache.copy_blocks([(0, 2), (1, 2)])
+    with pytest.raises(ValueError):
+        cache.copy_blocks([(0, 2), (2, 3)])
+
+
+def test_tree_masks():
+    mask, depth = tree_masks([[-1, 0, 0, 1], [-1], []])
+    assert mask.dtype == np.int64 and mask.tolist() == [[1], [3], [5], [11], [1]]
+    assert depth.tolist() == [0, 1, 1, 2, 0]
+    chain = [-1] + list(range(129))
+    mask, depth = tree_masks([chain])
+    assert mask.shape == (130, 3) and depth[-1] == 129
+    assert mask[63].tolist() == [-1, 0, 0] and mask[64].tolist() == [-1, 1, 0] and mask[129].tolist() == [-1, -1, 3]
+    assert tree_masks([])[0].shape == (0, 1)
+    for bad in ([0], [-1, 1], [-1, -1], [-1, 0, 3], [-1, -2]):
+        with pytest.raises(ValueError):
+            tree_masks([bad])
+    with pytest.raises(ValueError, match="256"):
+        tree_masks([[-1] + [0] * 256])
+
+
+def test_step_metadata_of_trees():
+    """Nodes take consecutive slots behind the context whatever their positions;
+    every node gets a logits row; no decode or prefill work remains."""
+    parents = [[-1, 0, 0, 1], [-1, 0]]
+    mask, depth = tree_masks(parents)
+    md = StepMeta([5, 6, 7, 8, 9, 10], [20, 21, 21, 22, 3, 4], [(0, 4), (4, 6)], [[9, 2], [4]], [24, 5], 16, 2,
+                  "cpu", pinned=False, all_logits=True, trees=mask)
+    assert md.slots.tolist() == [36, 37, 38, 39, 67, 68]          # positions 20..23 of block 2, 3..4 of 4
+    assert md.positions.tolist() == [20, 21, 21, 22, 3, 4] and md.ids.tolist() == [5, 6, 7, 8, 9, 10]
+    assert md.row_dst.tolist() == list(range(6)) and md.n_out == 6
+    assert md.n_dec == md.n_pre == 0 and md.n_tree == 2 and md.work.shape[0] == 0
+    assert md.tree_mask.tolist() == mask.tolist() and md.tree_bt.tolist() == [[9, 2], [4, -1]]
+    assert md.tree_q_start.tolist() == [0, 4] and md.tree_q_len.tolist() == [4, 2]
+    assert md.tree_ctx.tolist() == [24, 5] and (md.tree_max_q, md.tree_max_ctx, md.tree_ctx_sum) == (4, 24, 29)
+    with pytest.raises(IndexError):
+        StepMeta([1, 2], [16, 17], [(0, 2)], [[3]], [18], 16, 2, "cpu", pinned=False, trees=mask[:2])
+    with pytest.raises(ValueError):
+        StepMeta([1, 2], [0, 1], [(0, 2)], [[3]], [2], 16, 2, "cpu", pinned=False, trees=mask[:1])
+
+
+def test_fork_and_trim_tables():
+    bm = BlockManager(8, 4, False)
+    table, _ = bm.allocate_prompt(list(range(10)))                # 2 full blocks and half a third
+    fork, copies = bm.fork_table(table, 10)
+    assert fork[:2] == table[:2] and copies == [(table[2], fork[2])] and fork[2] not in table
+    assert [bm.blocks[b].ref_count for b in table] == [2, 2, 1] and bm.blocks[fork[2]].ref_count == 1
+    assert bm.blocks[fork[2]].token_ids == [8, 9]
+    whole, copies = bm.fork_table(table, 8)
+    assert whole == table[:2] and copies == [] and bm.blocks[table[0]].ref_count == 3
+    bm.free_table(whole)
+    # rejected drafts: blocks behind the kept tokens come back, shared ones stay with the other
+    fork += [bm._own(bm._fresh_block(), []).block_id for _ in range(2)]
+    assert bm.num_free() == 2
+    bm.trim_table(fork, 10)
+    assert len(fork) == 3 and bm.num_free() == 4
+    bm.trim_table(fork, 8)
+    bm.trim_table(fork, 8)
+    assert fork == table[:2] and bm.num_free() == 5
+    bm.trim_table(fork, 0)
+    assert fork == [] and [bm.blocks[b].ref_count for b in table] == [1, 1, 1]
+    bm.free_table(table)
+    assert bm.num_free() == 8
+    for bad in (-1, 1):
+        with pytest.raises(ValueError):
+            bm.fork_table([], bad)
+
+
+def test_fork_without_a_free_block_changes_nothing():
+    bm = BlockManager(2, 4, False)
+    table, _ = bm.allocate_prompt(list(range(6)))
+    with pytest.raises(OutOfBlocks):
+        bm.fork_table(table, 6)
+    assert [b.ref_count for b in bm.blocks] == [1, 1]
+
+
+def test_fork_keeps_prefix_cached_blocks_cached():
+    bm = BlockManager(4, 4, True)
+    table, _ = bm.allocate_prompt(list(range(8)))
+    fork, _ = bm.fork_table(table, 8)
+    bm.free_table(table)
+    assert bm.num_free() == 2
+    bm.free_table(fork)
+    assert bm.num_free() == 4 and bm.allocate_prompt(list(range(8)))[1] == 8
+
+
+def test_oracle_follows_the_target_exactly():
+    """The restatement's acceptance and residual, integrated over the draft and the
+    test's uniform number on a grid, give the target's distribution: two
+    siblings drawn without replacement from q, first emitted token."""
+    p = torch.tensor([.5, .2, .3], dtype=torch.float64)
+    q = torch.tensor([.2, .5, .3], dtype=torch.float64)
+    total = torch.zeros(3, dtype=torch.float64)
+    grid = 40
+    for a, b in itertools.permutations(range(3), 2):
+        weight = float(q[a] * q[b] / (1 - q[a]))
+        probs = torch.stack([p, p, p])
+        for i, j in itertools.product(range(grid), range(grid)):
+            for k in range(20):
+                u = torch.tensor([(k + .5) / 20, (i + .5) / grid, (j + .5) / grid], dtype=torch.float64)
+                took, path, nxt = R.verify([0, a, b], [-1, 0, 0], [0], [3], probs, u, 2, q[None],
+                                           torch.zeros(3, dtype=torch.int32))
+                tok = ([0, a, b][path[0][1]] if took[0] else nxt[0])
+                total[tok] += weight / (grid * grid * 20)
+                if took[0] and path[0][1] == 1:
+                    total[tok] += weight * 19 / (grid * grid * 20)
+                    break
+    # midpoint grids misplace a threshold by at most half a cell: two tests, one sample
+    assert bool(((total - p).abs() <= 2 * 0.5 / grid + 0.5 / 20).all()), total

@@ -8,7 +8,7 @@ stream is given.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_size_t, c_uint, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_size_t, c_uint, c_void_p
 from pathlib import Path
 
 import torch
@@ -67,6 +67,22 @@ _SIGS = {
     "tb_argmax": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "tb_argmax_vocab_parallel": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                          c_void_p, c_int, c_void_p]),
+    "tb_paged_attention_tree": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int,
+                                        c_int, c_int, c_int, c_int, c_void_p, c_int, c_int,
+                                        c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                        c_int, c_int, c_int, c_longlong, c_void_p]),
+    "tb_verify_drafts_greedy": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                        c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                        c_void_p, c_void_p]),
+    "tb_verify_drafts": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                 c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
+                                 c_void_p]),
+    "tb_keep_kv_path": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
+                                c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
+                                c_int, c_void_p]),
+    "tb_copy_kv_blocks": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
+                                  c_void_p]),
 }
 
 

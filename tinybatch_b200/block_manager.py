@@ -160,3 +160,32 @@ class BlockManager:
                 self.free_ids.append(bid)
             else:
                 self.evictable[bid] = None
+
+    # ------------------------------- forks and rejected drafts (no reference)
+
+    def fork_table(self, table: list[int], num_tokens: int) -> tuple[list[int], list[tuple[int, int]]]:
+        """A second table over the first ``num_tokens`` tokens of ``table``: full
+        blocks are shared, a partly filled last block gets a fresh copy of its
+        own.  Returns the table and the ``(source, destination)`` block copies
+        the caller has to make (``PagedKVCache.copy_blocks``) before either
+        sequence writes its next token."""
+        full, tail = divmod(num_tokens, self.block_size)
+        if num_tokens < 0 or full + (tail > 0) > len(table):
+            raise ValueError("the table does not hold that many tokens")
+        copies: list[tuple[int, int]] = []
+        new = list(table[:full])
+        if tail:
+            src = self.blocks[table[full]]
+            blk = self._own(self._fresh_block(), list(src.token_ids[:tail]))
+            copies.append((src.block_id, blk.block_id))
+            new.append(blk.block_id)
+        for bid in table[:full]:
+            self.blocks[bid].ref_count += 1
+        return new, copies
+
+    def trim_table(self, table: list[int], num_tokens: int) -> None:
+        """Release the blocks of ``table`` behind its first ``num_tokens`` tokens
+        (those that held rejected drafts), last first."""
+        keep = self.blocks_needed(num_tokens)
+        while len(table) > keep:
+            self.free_table([table.pop()])

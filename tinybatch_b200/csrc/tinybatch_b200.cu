@@ -7,3 +7,6 @@
 #include "capi.cu"
 #include "comm.cu"
 #include "static_scratch.cu"
+#include "tree_attention.cu"
+#include "verify.cu"
+#include "cache.cu"

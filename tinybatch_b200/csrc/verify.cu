@@ -1,0 +1,503 @@
+// Verification of drafted tokens.
+//
+// A sequence's draft tree has its nodes in the rows q_start .. q_start+q_len-1
+// of the flat batch; node 0 is the root (the last accepted token), parents[row]
+// < node index its parent inside the sequence.  The walk starts at the root and
+// goes from node to accepted child until no child is accepted.
+//
+// Greedy: the accepted child is the first one whose id is the target's argmax
+// at the node.
+//
+// Sampled: at node c with children x_1 .. x_m (node order), r_0 = probs[row c]
+// and, when the children were drawn without replacement from a distribution
+// d_0 = draft_probs[draft_rows[row c]]:
+//   x_j is accepted if d_{j-1}(x_j) > 0 and u_j d_{j-1}(x_j) < r_{j-1}(x_j);
+//   else r_j = max(r_{j-1} - d_{j-1}, 0) / Z_j, Z_j its sum (r_{j-1} kept where
+//   Z_j = 0), and d_j is d_0 without x_1 .. x_j over 1 - sum of their d_0.
+//   A child of draft probability 0 is rejected and changes nothing.
+// Children picked outright (draft row -1): x_j is accepted if
+//   r(x_j) > 0 and u_j (1 - sum of the rejected r) < r(x_j), else r(x_j) becomes 0.
+// When no child is accepted the next token is the first y whose cumulative
+// sum of r exceeds u_root * sum(r).  With u uniform this leaves the target's
+// distribution unchanged (speculative sampling; Leviathan et al. 2023, with
+// several candidates a node as in Miao et al. 2024).
+//
+// Everything is evaluated in 64 bits: the tests compare products of 24-bit
+// numbers, and the position of a sample among ~1.5e5 cumulative sums would
+// move with the summation order in 32.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "host.h"
+
+namespace tb {
+
+constexpr int VF_NODES = 256;      // nodes of a sequence's tree
+constexpr int VF_THREADS = 512;
+constexpr int VF_WARPS = VF_THREADS / 32;
+constexpr int VF_MAX_CLUSTER = 8;
+
+struct TreeArgs {
+  const int *ids, *parents, *q_start, *q_len;
+  int n_seqs, n_rows;
+  int *n_accepted, *path, *next_ids;
+  int path_ld, path_w;
+};
+
+struct VerifyArgs {
+  TreeArgs t;
+  const float* probs;
+  long long ld_p;
+  int vocab;
+  const float* draft_probs;
+  long long ld_d;
+  int n_draft_rows;
+  const int* draft_rows;
+  const float* uniforms;
+};
+
+// The rows of sequence `seq` lie inside the batch and its tree is not too large.
+__device__ __forceinline__ bool tree_ok(const TreeArgs& t, int q0, int ql) {
+  return ql >= 0 && ql <= VF_NODES && q0 >= 0 && q0 <= t.n_rows - ql;
+}
+
+// ------------------------------------------------------------------- greedy
+
+constexpr int VG_WARPS = 4;
+
+// One warp a sequence: its nodes in shared memory, then one ballot round a step.
+__global__ void __launch_bounds__(VG_WARPS * 32)
+    verify_greedy_kernel(const TreeArgs t, const int* target_ids) {
+  __shared__ int s_par[VG_WARPS][VF_NODES], s_id[VG_WARPS][VF_NODES], s_tgt[VG_WARPS][VF_NODES];
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int seq = blockIdx.x * VG_WARPS + warp;
+  if (seq >= t.n_seqs) return;
+  const int q0 = t.q_start[seq], ql = t.q_len[seq];
+  int* path = t.path + (size_t)seq * t.path_ld;
+  int n = 0, next = -1;
+  if (!tree_ok(t, q0, ql)) {
+    if (lane == 0) set_status(ERR_BAD_INDEX);
+  } else if (ql > 0) {
+    for (int i = lane; i < ql; i += 32) {
+      int p = t.parents[q0 + i];
+      if (i > 0 && (p < 0 || p >= i)) {   // unreachable
+        set_status(ERR_BAD_INDEX);
+        p = -1;
+      }
+      s_par[warp][i] = i > 0 ? p : -1;
+      s_id[warp][i] = t.ids[q0 + i];
+      s_tgt[warp][i] = target_ids[q0 + i];
+    }
+    __syncwarp();
+    int c = 0;
+    if (lane == 0) path[0] = 0;
+    n = 1;
+    next = s_tgt[warp][0];
+    while (n < t.path_w) {
+      int found = -1;
+      for (int i0 = c & ~31; i0 < ql && found < 0; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned hit = __ballot_sync(
+            0xffffffffu, i < ql && s_par[warp][i] == c && s_id[warp][i] == next);
+        if (hit) found = i0 + __ffs(hit) - 1;
+      }
+      if (found < 0) break;
+      c = found;
+      if (lane == 0) path[n] = c;
+      ++n;
+      next = s_tgt[warp][c];
+    }
+  }
+  for (int k = n + lane; k < t.path_w; k += 32) path[k] = -1;
+  if (lane == 0) {
+    t.n_accepted[seq] = n > 0 ? n - 1 : 0;
+    t.next_ids[seq] = next;
+  }
+}
+
+// ------------------------------------------------------------------ sampled
+
+// What has been rejected at the current node, in order.
+struct Rejections {
+  int n;                      // entries
+  int token[VF_NODES];
+  double scale[VF_NODES];     // draft distribution: 1 / (1 - sum of d_0 of earlier entries)
+  double inv_z[VF_NODES];     // 1 / Z, or 0 where Z was 0 (r kept)
+};
+
+// r after every rejection of h at a token with target probability p and draft
+// probability d; `special`: the token is among the rejected ones.
+template <bool DIST>
+__device__ __forceinline__ double residual(const Rejections& h, int token, float p, float d,
+                                           bool special) {
+  double r = p;
+  if (DIST) {
+    double dd = d;
+    for (int k = 0; k < h.n; ++k) {
+      const double iz = h.inv_z[k];
+      if (iz > 0.0) r = fmax(r - dd * h.scale[k], 0.0) * iz;
+      if (special && h.token[k] == token) dd = 0.0;
+    }
+  } else if (special) {
+    for (int k = 0; k < h.n; ++k)
+      if (h.token[k] == token) r = 0.0;
+  }
+  return r;
+}
+
+__device__ __forceinline__ bool rejected(const Rejections& h, int first, int count) {
+  bool s = false;
+  for (int k = 0; k < h.n; ++k) s |= (unsigned)(h.token[k] - first) < (unsigned)count;
+  return s;
+}
+
+// r of the four consecutive tokens from y on (0 from `end` on).
+template <bool DIST>
+__device__ __forceinline__ void residual4(const Rejections& h, const float* p, const float* d,
+                                          int y, int end, bool vec, double* w) {
+  float pv[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
+  if (vec && y + 4 <= end) {
+    const float4 a = *reinterpret_cast<const float4*>(p + y);
+    pv[0] = a.x, pv[1] = a.y, pv[2] = a.z, pv[3] = a.w;
+    if (DIST) {
+      const float4 b = *reinterpret_cast<const float4*>(d + y);
+      dv[0] = b.x, dv[1] = b.y, dv[2] = b.z, dv[3] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (y + e < end) {
+        pv[e] = p[y + e];
+        if (DIST) dv[e] = d[y + e];
+      }
+  }
+  const bool special = rejected(h, y, 4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = residual<DIST>(h, y + e, pv[e], dv[e], special);
+}
+
+// One cluster a sequence, the vocabulary cut into one segment a warp.  Every
+// CTA walks the tree alike (same loads, same arithmetic), so the cluster only
+// meets for sums over the vocabulary: one after each rejection that has to
+// know Z, one for the sample.
+__global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) {
+  namespace cg = cooperative_groups;
+  __shared__ int s_id[VF_NODES], s_first[VF_NODES], s_sib[VF_NODES], s_par[VF_NODES];
+  __shared__ float s_p[VF_NODES], s_d[VF_NODES], s_u[VF_NODES];
+  __shared__ int s_drow[VF_NODES];
+  __shared__ Rejections s_h;
+  __shared__ double s_sum[2][VF_MAX_CLUSTER * VF_WARPS];
+  __shared__ double s_prefix[VF_MAX_CLUSTER + 1];
+  cg::cluster_group cluster = cg::this_cluster();
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_trigger();
+  const TreeArgs& t = a.t;
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int seq = blockIdx.x / C;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int q0 = t.q_start[seq], ql = t.q_len[seq];
+  int* path = t.path + (size_t)seq * t.path_ld;
+  const bool ok = tree_ok(t, q0, ql);
+  if (!ok || ql == 0) {   // uniform over the cluster
+    if (rank == 0) {
+      if (!ok && tid == 0) set_status(ERR_BAD_INDEX);
+      for (int k = tid; k < t.path_w; k += VF_THREADS) path[k] = -1;
+      if (tid == 0) {
+        t.n_accepted[seq] = 0;
+        t.next_ids[seq] = -1;
+      }
+    }
+    return;
+  }
+
+  auto started = cluster.barrier_arrive();   // waited for before the first remote store
+
+  // ---- the tree and, for every node, the probabilities its test compares
+  for (int i = tid; i < ql; i += VF_THREADS) {
+    int p = t.parents[q0 + i];
+    const int id = t.ids[q0 + i];
+    int dr = a.draft_rows != nullptr ? a.draft_rows[q0 + i] : -1;
+    if (dr >= a.n_draft_rows || dr < -1) {
+      set_status(ERR_BAD_INDEX);
+      dr = -1;
+    }
+    if (i == 0) {
+      p = -1;
+    } else if (p < 0 || p >= i || id < 0 || id >= a.vocab) {   // unreachable
+      set_status(ERR_BAD_INDEX);
+      p = -1;
+    }
+    s_par[i] = p;
+    s_id[i] = id;
+    s_u[i] = a.uniforms[q0 + i];
+    s_drow[i] = dr;
+    s_first[i] = VF_NODES;
+    s_p[i] = p >= 0 ? a.probs[(size_t)(q0 + p) * a.ld_p + id] : 0.f;
+  }
+  __syncthreads();
+  for (int i = tid; i < ql; i += VF_THREADS) {
+    const int p = s_par[i];
+    int sib = VF_NODES;
+    if (p >= 0) {
+      atomicMin(&s_first[p], i);
+      const int dr = s_drow[p];
+      s_d[i] = dr >= 0 ? a.draft_probs[(size_t)dr * a.ld_d + s_id[i]] : 0.f;
+      for (int j = i + 1; j < ql; ++j)
+        if (s_par[j] == p) {
+          sib = j;
+          break;
+        }
+    }
+    s_sib[i] = sib;
+  }
+  if (tid == 0) s_h.n = 0;
+  __syncthreads();
+  cluster.barrier_wait(std::move(started));
+
+  // this warp's segment of the vocabulary
+  const int n_seg = C * VF_WARPS;
+  const int seg_len = ((a.vocab + n_seg * 128 - 1) / (n_seg * 128)) * 128;
+  const int seg = rank * VF_WARPS + warp;
+  const long long y_begin = (long long)seg * seg_len;
+  const int y0 = y_begin < a.vocab ? (int)y_begin : a.vocab;
+  const int y1 = y_begin + seg_len < a.vocab ? (int)(y_begin + seg_len) : a.vocab;
+  const bool vec_p = a.ld_p % 4 == 0 && reinterpret_cast<uintptr_t>(a.probs) % 16 == 0;
+  const bool vec_d = a.ld_d % 4 == 0 && reinterpret_cast<uintptr_t>(a.draft_probs) % 16 == 0;
+  int parity = 0;
+  double* sums = s_sum[0];
+
+  // Sum over the vocabulary of r with the rejections of s_h applied.  All
+  // threads of the cluster call it; every one gets the same sum.  s_prefix:
+  // the CTAs' exclusive prefix sums, summed in rank order (so they never
+  // decrease), and the total.
+  auto vocab_sum = [&](const float* p, const float* d, bool dist) -> double {
+    double acc = 0.0;
+    const bool vec = vec_p && (!dist || vec_d);
+    for (int y = y0 + 4 * lane; y < y1; y += 128) {
+      double w[4];
+      if (dist) residual4<true>(s_h, p, d, y, y1, vec, w);
+      else residual4<false>(s_h, p, d, y, y1, vec, w);
+      acc += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    sums = s_sum[parity];
+    if (lane < C) cluster.map_shared_rank(sums, lane)[seg] = acc;
+    cluster.sync();
+    if (warp == 0) {
+      double s = 0.0;
+      if (lane < C)
+#pragma unroll
+        for (int k = 0; k < VF_WARPS; ++k) s += sums[lane * VF_WARPS + k];
+      double run = 0.0;
+      for (int k = 0; k < C; ++k) {
+        if (lane == 0) s_prefix[k] = run;
+        run += __shfl_sync(0xffffffffu, s, k);
+      }
+      if (lane == 0) s_prefix[C] = run;
+    }
+    __syncthreads();
+    parity ^= 1;   // the other buffer: a CTA may still be reading this one
+    return s_prefix[C];
+  };
+
+  // ---- the walk
+  int c = 0, n = 1;
+  bool dist = false;
+  const float* prow = a.probs;
+  const float* drow = nullptr;
+  if (rank == 0 && tid == 0) path[0] = 0;
+  while (true) {
+    prow = a.probs + (size_t)(q0 + c) * a.ld_p;
+    dist = s_drow[c] >= 0;
+    drow = dist ? a.draft_probs + (size_t)s_drow[c] * a.ld_d : nullptr;
+    double gone = 0.0;
+    int took = -1;
+    for (int x = n < t.path_w ? s_first[c] : VF_NODES; x < VF_NODES; x = s_sib[x]) {
+      const int id = s_id[x];
+      const double u = s_u[x];
+      const bool again = rejected(s_h, id, 1);
+      bool changes = true;
+      if (dist) {
+        const double left = 1.0 - gone;
+        const double scale = left > 0.0 ? 1.0 / left : 0.0;
+        const double share = again ? 0.0 : s_d[x] * scale;
+        if (share > 0.0) {
+          const double r = residual<true>(s_h, id, s_p[x], s_d[x], again);
+          if (u * share < r) took = x;
+        } else {
+          changes = false;
+        }
+        if (took < 0 && changes) {
+          __syncthreads();          // every thread has read s_h
+          if (tid == 0) {
+            s_h.token[s_h.n] = id;
+            s_h.scale[s_h.n] = scale;
+            s_h.inv_z[s_h.n] = 1.0;
+            s_h.n += 1;
+          }
+          __syncthreads();
+          const double z = vocab_sum(prow, drow, true);
+          if (tid == 0) s_h.inv_z[s_h.n - 1] = z > 0.0 ? 1.0 / z : 0.0;
+          __syncthreads();
+          gone += s_d[x];
+        }
+      } else {
+        const double r = again ? 0.0 : (double)s_p[x];
+        if (r > 0.0 && u * (1.0 - gone) < r) took = x;
+        else {
+          gone += r;
+          __syncthreads();
+          if (tid == 0) {
+            s_h.token[s_h.n] = id;
+            s_h.n += 1;
+          }
+          __syncthreads();
+        }
+      }
+      if (took >= 0) break;
+    }
+    if (took < 0) break;
+    c = took;
+    if (rank == 0 && tid == 0) path[n] = c;
+    ++n;
+    __syncthreads();
+    if (tid == 0) s_h.n = 0;
+    __syncthreads();
+  }
+
+  // ---- the sample: the CTA, then its warp, then the element in which the
+  // cumulative sum passes the target.  Each level searches its own running
+  // sums, so exactly one warp answers; a target that rounding leaves past a
+  // level's last sum takes the last positive one.
+  const double total = vocab_sum(prow, drow, dist);
+  if (rank == 0) {
+    for (int k = n + tid; k < t.path_w; k += VF_THREADS) path[k] = -1;
+    if (tid == 0) {
+      t.n_accepted[seq] = n - 1;
+      if (!(total > 0.0)) t.next_ids[seq] = -1;
+    }
+  }
+  if (!(total > 0.0)) return;
+  const double aim = fmax((double)s_u[0] * total, 0.0);   // a NaN aims at 0
+  const double lo = s_prefix[rank], hi = s_prefix[rank + 1];
+  if (!(lo < hi && ((lo <= aim && aim < hi) || (aim >= total && hi >= total)))) return;
+  double at = aim - lo, run = 0.0;
+  int mine = 0;
+  double before = 0.0;
+  for (int w = 0; w < VF_WARPS; ++w) {
+    const double s = sums[rank * VF_WARPS + w];
+    if (!(s > 0.0)) continue;
+    mine = w;
+    before = run;
+    run += s;
+    if (at < run) break;
+  }
+  if (warp != mine) return;
+  at -= before;
+  run = 0.0;
+  const bool vec = vec_p && (!dist || vec_d);
+  int next = -1;
+  for (int y = y0 + 4 * lane; y - 4 * lane < y1; y += 128) {
+    double w[4];
+    if (dist) residual4<true>(s_h, prow, drow, y, y1, vec, w);
+    else residual4<false>(s_h, prow, drow, y, y1, vec, w);
+    const double sum = (w[0] + w[1]) + (w[2] + w[3]);
+    double inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    double cum = __shfl_up_sync(0xffffffffu, inc, 1);
+    cum = run + (lane > 0 ? cum : 0.0);
+    int hit = -1, pos = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      cum += w[e];
+      if (w[e] > 0.0) {
+        pos = y + e;
+        if (hit < 0 && cum > at) hit = y + e;
+      }
+    }
+    const unsigned some = __ballot_sync(0xffffffffu, pos >= 0);
+    if (some) next = __shfl_sync(0xffffffffu, pos, 31 - __clz(some));
+    const unsigned any = __ballot_sync(0xffffffffu, hit >= 0);
+    if (any) {
+      next = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
+      break;
+    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) t.next_ids[seq] = next;
+}
+
+static int check_tree(const TreeArgs& t, int max_q) {
+  if (t.n_seqs < 0 || t.n_rows < 0 || t.path_w <= 0 || t.path_ld < t.path_w)
+    return arg_err("n_seqs / n_rows / path width");
+  if (max_q > VF_NODES) return arg_err("a draft tree has at most 256 nodes");
+  if (t.n_seqs > 0 && (t.ids == nullptr || t.parents == nullptr || t.q_start == nullptr ||
+                       t.q_len == nullptr || t.n_accepted == nullptr || t.path == nullptr ||
+                       t.next_ids == nullptr))
+    return arg_err("null pointer");
+  return TB_OK;
+}
+
+int verify_greedy_launch(const TreeArgs& t, const int* target_ids, int max_q, cudaStream_t st) {
+  if (int rc = check_tree(t, max_q)) return rc;
+  if (t.n_seqs == 0) return TB_OK;
+  if (target_ids == nullptr) return arg_err("null pointer");
+  return launch_pdl(verify_greedy_kernel, dim3((t.n_seqs + VG_WARPS - 1) / VG_WARPS),
+                    dim3(VG_WARPS * 32), 0, st, 1, "greedy verification launch", t, target_ids);
+}
+
+int verify_launch(const VerifyArgs& a, int max_q, cudaStream_t st) {
+  if (int rc = check_tree(a.t, max_q)) return rc;
+  if (a.t.n_seqs == 0) return TB_OK;
+  if (a.vocab <= 0 || a.ld_p < a.vocab || a.probs == nullptr || a.uniforms == nullptr)
+    return arg_err("probs / vocab / uniforms");
+  if ((a.draft_probs == nullptr) != (a.draft_rows == nullptr))
+    return arg_err("draft_probs and draft_rows go together");
+  if (a.draft_probs != nullptr && (a.ld_d < a.vocab || a.n_draft_rows < 0))
+    return arg_err("draft_probs shape");
+  const int cluster = VF_MAX_CLUSTER;
+  if (a.t.n_seqs > 0x7fffffff / cluster) return arg_err("n_seqs");
+  return launch_pdl(verify_kernel, dim3(a.t.n_seqs * cluster), dim3(VF_THREADS), 0, st, cluster,
+                    "draft verification launch", a);
+}
+
+}  // namespace tb
+
+extern "C" {
+
+int tb_verify_drafts_greedy(const int* ids, const int* parents, const int* q_start,
+                            const int* q_len, int n_seqs, int n_rows, int max_q,
+                            const int* target_ids, int* n_accepted, int* path, int path_ld,
+                            int path_w, int* next_ids, void* stream) {
+  const tb::TreeArgs t{ids, parents, q_start, q_len, n_seqs, n_rows,
+                       n_accepted, path, next_ids, path_ld, path_w};
+  return tb::verify_greedy_launch(t, target_ids, max_q, static_cast<cudaStream_t>(stream));
+}
+
+int tb_verify_drafts(const int* ids, const int* parents, const int* q_start, const int* q_len,
+                     int n_seqs, int n_rows, int max_q, const float* probs, long long ld_probs,
+                     int vocab, const float* draft_probs, long long ld_draft, int n_draft_rows,
+                     const int* draft_rows, const float* uniforms, int* n_accepted, int* path,
+                     int path_ld, int path_w, int* next_ids, void* stream) {
+  tb::VerifyArgs a{};
+  a.t = tb::TreeArgs{ids, parents, q_start, q_len, n_seqs, n_rows,
+                     n_accepted, path, next_ids, path_ld, path_w};
+  a.probs = probs;
+  a.ld_p = ld_probs;
+  a.vocab = vocab;
+  a.draft_probs = draft_probs;
+  a.ld_d = ld_draft;
+  a.n_draft_rows = n_draft_rows;
+  a.draft_rows = draft_rows;
+  a.uniforms = uniforms;
+  return tb::verify_launch(a, max_q, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -11,10 +11,16 @@ On the hot path nothing here runs: the fused QKV kernel writes K/V straight
 into the pools and the attention kernel reads them through the block tables.
 ``write`` and ``gather`` keep the reference's methods for callers and tests;
 they are plain device tensor indexing.
+
+``copy_blocks`` (forks, moves of whole blocks) and ``keep_path`` (the accepted
+path of a verified draft tree) are kernels over all layers at once; the
+reference has neither.
 """
 from __future__ import annotations
 
 import torch
+
+from . import ops
 
 
 class PagedKVCache:
@@ -27,6 +33,36 @@ class PagedKVCache:
         self.head_dim = head_dim
         self.pools = [torch.zeros(num_blocks, 2, n_kv_heads, block_size, head_dim,
                                   device=device, dtype=dtype) for _ in range(n_layers)]
+
+        self._handle: ops.KVPools | None = None
+
+    def handle(self) -> ops.KVPools:
+        """The pools as one argument of ``ops.keep_kv_path`` / ``copy_kv_blocks``."""
+        h = self._handle
+        if h is None or len(h.pools) != len(self.pools) or any(
+                a is not b for a, b in zip(h.pools, self.pools)):
+            h = self._handle = ops.KVPools(self.pools)
+        return h
+
+    def copy_blocks(self, pairs: list[tuple[int, int]]) -> None:
+        """Copy whole blocks, ``(source, destination)`` ids, in every layer
+        (the copies ``BlockManager.fork_table`` asks for)."""
+        pairs = [(int(a), int(b)) for a, b in pairs]
+        if not pairs:
+            return
+        src, dst = [a for a, _ in pairs], [b for _, b in pairs]
+        if any(not 0 <= b < self.num_blocks for b in src + dst):
+            raise IndexError("block id out of range")
+        if len(set(dst)) != len(dst) or set(dst) & set(src):
+            raise ValueError("a destination block is written twice or is also a source")
+        host = torch.tensor(pairs, dtype=torch.int32).pin_memory()
+        ops.copy_kv_blocks(self.handle(), host.to(self.pools[0].device, non_blocking=True))
+
+    def keep_path(self, *, block_tables, q_len, ctx_len, path, n_accepted) -> None:
+        """Move the K/V of the accepted draft nodes to consecutive positions
+        (``ops.keep_kv_path`` over this cache's pools)."""
+        ops.keep_kv_path(self.handle(), block_tables=block_tables, q_len=q_len, ctx_len=ctx_len,
+                         path=path, n_accepted=n_accepted)
 
     def memory_bytes(self) -> int:
         return sum(p.numel() * p.element_size() for p in self.pools)

@@ -16,7 +16,7 @@ import torch
 from . import _native
 from .config import ModelConfig
 from .kv_cache import PagedKVCache
-from .runtime import DeviceModel, RankWeights, StepMeta
+from .runtime import DeviceModel, RankWeights, StepMeta, tree_masks
 
 
 def _to_list(x):
@@ -86,3 +86,37 @@ class Qwen2Paged:
         """Forward over prebuilt metadata; logits stay in the model's buffer
         (valid until the next call)."""
         return self.dm.forward(md, kv_cache.pools, sample=sample)
+
+    @torch.inference_mode()
+    def forward_tree(self, token_ids, parents, block_tables, context_lens,
+                     kv_cache: PagedKVCache, sample: bool = False):
+        """Forward over draft trees (speculative decoding): one tree a sequence,
+        ``parents[s]`` the parent of each of its nodes (-1 for node 0, the last
+        accepted token; see ``runtime.tree_masks``), ``token_ids`` the nodes of
+        all trees one after another, ``context_lens[s]`` the tokens of the
+        sequence with its nodes.  Node i's K/V go to position ``context - nodes
+        + i`` of the block table; its rotary position is the root's plus its
+        depth.  Returns the metadata and the logits after every node ``[rows,
+        vocab]``, or with ``sample`` the target's greedy choice after every
+        node ``[rows]``; both stay in the model's buffers until the next call.
+        ``ops.verify_drafts*`` take it from there with ``md.tree_q_start`` and
+        ``md.tree_q_len``."""
+        if self.world != 1:
+            raise RuntimeError("forward_tree runs on one rank")
+        parents = [_to_list(p) for p in parents]
+        ctx = _to_list(context_lens)
+        if len(ctx) != len(parents):
+            raise ValueError("one context length per tree")
+        mask, depth = tree_masks(parents)
+        slices, pos, r0 = [], [], 0
+        for par, c in zip(parents, ctx):
+            if not par or c < len(par):
+                raise ValueError("every tree has a root and its context holds its nodes")
+            slices.append((r0, r0 + len(par)))
+            pos += [c - len(par) + int(d) for d in depth[r0:r0 + len(par)]]
+            r0 += len(par)
+        md = StepMeta(_to_list(token_ids), pos, slices, [list(t) for t in block_tables], ctx,
+                      kv_cache.block_size, self.cfg.n_heads // self.cfg.n_kv_heads, self.device,
+                      all_logits=True, trees=mask)
+        logits = self.dm.forward(md, kv_cache.pools, sample=sample)
+        return md, (self.dm.next_ids[:md.T] if sample else logits)

@@ -7,6 +7,8 @@ allocates per call except when no arena is given).
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _native as N
@@ -152,6 +154,222 @@ def paged_attention_prefill(q, out, kv_pool, *, n_q_heads, n_kv_heads, head_dim,
         "tb_paged_attention_prefill")
 
 
+# ------------------------------------------------- speculative decoding
+#
+# These calls check types, shapes, devices and strides of every tensor (a
+# mistake raises ValueError before anything is launched) and run on the
+# tensors' own device, on its current stream.
+
+def _device(t: torch.Tensor) -> int:
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError("expected CUDA tensors")
+    return dev
+
+
+def _in(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev: int) -> int:
+    """Data pointer of an argument of the given type, shape (None: any size)
+    and device whose last dimension is contiguous."""
+    got = t.shape
+    if t.dtype is not dtype or t.get_device() != dev or len(got) != len(shape):
+        raise ValueError(f"{name}: expected a {len(shape)}-d {dtype} tensor on cuda:{dev}, got "
+                         f"{tuple(got)} {t.dtype} on {t.device}")
+    for g, w in zip(got, shape):
+        if w is not None and g != w:
+            raise ValueError(f"{name}: expected shape {shape}, got {tuple(got)}")
+    if got and got[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return t.data_ptr()
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row pitch of a 2-d argument in elements (its width where it has one row)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _run_on(dev: int, what: str, fn, *args) -> None:
+    """Call ``fn(*args, stream)`` on device ``dev``'s current stream."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        N.check(rc, what)
+
+
+def paged_attention_tree(q, out, kv_pool, *, n_q_heads, n_kv_heads, head_dim, block_size,
+                         block_tables, q_start, q_len, ctx_len, tree_mask, max_q=None,
+                         max_ctx=0, ctx_total=0):
+    """Attention of drafted tokens over the paged cache: row ``q_start[s] + i``
+    is node i of sequence s's draft tree, its K/V at position ``ctx_len[s] -
+    q_len[s] + i``; it sees every earlier position and the nodes whose bits
+    are set in its row of ``tree_mask`` (int64 ``[rows, words]``, bit ``j %
+    64`` of word ``j // 64``; ``runtime.tree_masks`` builds it).  Rows that
+    see nothing get zeros, rows of no sequence are left as they were.
+
+    ``max_q``: the largest ``q_len`` (default: as many as the mask can name).
+    ``max_ctx`` / ``ctx_total``: the longest context and their sum where the
+    caller knows them (they only choose how a context is shared out)."""
+    lib = N.load()
+    dev = _device(q)
+    rows = q.shape[0]
+    n = ctx_len.shape[0]
+    words = tree_mask.shape[-1]
+    bf = torch.bfloat16
+    width = n_q_heads * head_dim
+    qp = _in("q", q, bf, (rows, width), dev)
+    op = _in("out", out, bf, (rows, width), dev)
+    pp = _in("kv_pool", kv_pool, bf, (None, 2, n_kv_heads, block_size, head_dim), dev)
+    if not kv_pool.is_contiguous():
+        raise ValueError("kv_pool must be contiguous")
+    i32 = torch.int32
+    bp = _in("block_tables", block_tables, i32, (n, None), dev)
+    sp = _in("q_start", q_start, i32, (n,), dev)
+    lp = _in("q_len", q_len, i32, (n,), dev)
+    cp = _in("ctx_len", ctx_len, i32, (n,), dev)
+    mp = _in("tree_mask", tree_mask, torch.int64, (rows, words), dev)
+    if max_q is None:
+        max_q = min(rows, 64 * words)
+    _run_on(dev, "tb_paged_attention_tree", lib.tb_paged_attention_tree, qp, _ld(q), op, _ld(out),
+            rows, pp, kv_pool.shape[0], n_q_heads, n_kv_heads, head_dim, block_size, bp,
+            _ld(block_tables), block_tables.shape[1], sp, lp, cp, n, mp, _ld(tree_mask), words,
+            max_q, max_ctx, ctx_total)
+
+
+def _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev):
+    """Pointers and sizes of the arguments both verifications share."""
+    i32 = torch.int32
+    rows, n = ids.shape[0], q_len.shape[0]
+    return (rows, n,
+            (_in("ids", ids, i32, (rows,), dev), _in("parents", parents, i32, (rows,), dev),
+             _in("q_start", q_start, i32, (n,), dev), _in("q_len", q_len, i32, (n,), dev)),
+            (_in("n_accepted", n_accepted, i32, (n,), dev), _in("path", path, i32, (n, None), dev),
+             _ld(path), path.shape[1], _in("next_ids", next_ids, i32, (n,), dev)))
+
+
+def verify_drafts_greedy(ids, parents, q_start, q_len, target_ids, n_accepted, path, next_ids, *,
+                         max_q=0):
+    """Walk every sequence's draft tree along the target's choices: from the
+    root to the first child whose id is ``target_ids`` at its parent's row, as
+    long as there is one.  Writes the accepted nodes (root first, then -1) to
+    ``path`` ``[n, width]``, how many drafts they are to ``n_accepted`` and
+    the target's choice after the last of them to ``next_ids``."""
+    lib = N.load()
+    dev = _device(ids)
+    rows, n, tree, outs = _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev)
+    tp = _in("target_ids", target_ids, torch.int32, (rows,), dev)
+    _run_on(dev, "tb_verify_drafts_greedy", lib.tb_verify_drafts_greedy, *tree, n, rows, max_q, tp,
+            *outs)
+
+
+def verify_drafts(ids, parents, q_start, q_len, probs, uniforms, n_accepted, path, next_ids, *,
+                  draft_probs=None, draft_rows=None, max_q=0):
+    """Verify draft trees by speculative sampling, so that the accepted tokens
+    and ``next_ids`` follow the target's distribution.
+
+    ``probs`` ``[rows, vocab]`` fp32: the target's distribution after each
+    node.  ``draft_probs`` ``[k, vocab]`` fp32 with ``draft_rows`` ``[rows]``
+    int32: the distribution each node's children were drawn from without
+    replacement (-1, or both None: picked outright).  ``uniforms`` ``[rows]``
+    fp32 in [0, 1): one for each draft's test, the root's for the final
+    sample.  Outputs as ``verify_drafts_greedy``."""
+    lib = N.load()
+    dev = _device(ids)
+    rows, n, tree, outs = _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev)
+    f32 = torch.float32
+    pp = _in("probs", probs, f32, (rows, None), dev)
+    up = _in("uniforms", uniforms, f32, (rows,), dev)
+    vocab = probs.shape[1]
+    if (draft_probs is None) != (draft_rows is None):
+        raise ValueError("draft_probs and draft_rows go together")
+    draft = (None, 0, 0, None)
+    if draft_probs is not None:
+        draft = (_in("draft_probs", draft_probs, f32, (None, vocab), dev), _ld(draft_probs),
+                 draft_probs.shape[0], _in("draft_rows", draft_rows, torch.int32, (rows,), dev))
+    _run_on(dev, "tb_verify_drafts", lib.tb_verify_drafts, *tree, n, rows, max_q, pp, _ld(probs),
+            vocab, *draft, up, *outs)
+
+
+class KVPools:
+    """The layers' KV pools as one argument of the cache moves: checked once,
+    their addresses in a host array.  Holds the tensors."""
+
+    def __init__(self, pools):
+        """``pools``: a list of ``[num_blocks, 2, n_kv, block_size, head_dim]``
+        bf16 tensors, or one tensor with the layers stacked in front."""
+        stacked = isinstance(pools, torch.Tensor)
+        if stacked and pools.dim() != 6:
+            raise ValueError("stacked pools: expected [layers, num_blocks, 2, n_kv, block_size, head_dim]")
+        if not stacked:
+            pools = list(pools)
+        self.pools = pools
+        self.n_layers = len(pools)
+        if self.n_layers == 0:
+            raise ValueError("no pools")
+        first = pools[0]
+        self.device = _device(first)
+        shape = first.shape
+        if len(shape) != 5 or shape[1] != 2:
+            raise ValueError(f"pools: expected [num_blocks, 2, n_kv, block_size, head_dim], got {tuple(shape)}")
+        if stacked:
+            if first.dtype is not torch.bfloat16 or not first.is_contiguous():
+                raise ValueError("pools must be bf16 and contiguous")
+            step = pools.stride(0) * 2
+            if self.n_layers > 1 and step < first.numel() * 2:
+                raise ValueError("pools: layers overlap")
+            p0 = first.data_ptr()
+            ptrs = [p0 + i * step for i in range(self.n_layers)]
+        else:
+            for t in pools:
+                if (t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous()
+                        or t.get_device() != self.device):
+                    raise ValueError("pools must be contiguous bf16 tensors of one shape and device")
+            ptrs = [t.data_ptr() for t in pools]
+            if len(set(ptrs)) != len(ptrs):
+                raise ValueError("pools: a layer is listed twice")
+        self.num_blocks, _, self.n_kv_heads, self.block_size, self.head_dim = shape
+        self.array = (ctypes.c_void_p * self.n_layers)(*ptrs)
+        self.args = (self.array, self.n_layers, *(int(shape[i]) for i in (0, 2, 3, 4)))
+
+
+def _pools(pools) -> KVPools:
+    return pools if isinstance(pools, KVPools) else KVPools(pools)
+
+
+def keep_kv_path(pools, *, block_tables, q_len, ctx_len, path, n_accepted):
+    """After a verification: in every layer, move the K/V of each sequence's
+    accepted nodes (``path``, ``n_accepted`` as the verification wrote them)
+    to the consecutive positions after the root.  ``pools``: ``KVPools``, or
+    what it takes."""
+    lib = N.load()
+    kv = _pools(pools)
+    dev = kv.device
+    i32 = torch.int32
+    n = q_len.shape[0]
+    bp = _in("block_tables", block_tables, i32, (n, None), dev)
+    lp = _in("q_len", q_len, i32, (n,), dev)
+    cp = _in("ctx_len", ctx_len, i32, (n,), dev)
+    pp = _in("path", path, i32, (n, None), dev)
+    ap = _in("n_accepted", n_accepted, i32, (n,), dev)
+    _run_on(dev, "tb_keep_kv_path", lib.tb_keep_kv_path, *kv.args, bp, _ld(block_tables),
+            block_tables.shape[1], lp, cp, pp, _ld(path), path.shape[1], ap, n)
+
+
+def copy_kv_blocks(pools, pairs):
+    """Copy block ``pairs[i, 0]`` to block ``pairs[i, 1]`` in every layer
+    (``pairs`` int32 ``[n, 2]`` on the device).  No destination may be
+    another pair's source or destination: such pairs are not made and set the
+    status word.  ``pools``: ``KVPools``, or what it takes."""
+    lib = N.load()
+    kv = _pools(pools)
+    pp = _in("pairs", pairs, torch.int32, (None, 2), kv.device)
+    if not pairs.is_contiguous():
+        raise ValueError("pairs must be contiguous")
+    _run_on(kv.device, "tb_copy_kv_blocks", lib.tb_copy_kv_blocks, *kv.args, pp, pairs.shape[0])
+
+
 def embed(ids, emb, g, h, hg, sq):
     lib = N.load()
     M = ids.shape[0]
@@ -169,7 +387,6 @@ def argmax(logits, out):
 
 
 def max_active_clusters(bn: int, cluster: int) -> int:
-    import ctypes
     out = ctypes.c_int(0)
     N.check(N.load().tb_gemm_max_active_clusters(bn, cluster, ctypes.byref(out)),
             "tb_gemm_max_active_clusters")

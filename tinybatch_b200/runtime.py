@@ -257,6 +257,34 @@ def prefill_work(q_len, ctx, group: int) -> np.ndarray:
     return np.asarray([items[i] for i in order], dtype=np.int32).reshape(-1, 2)
 
 
+TREE_MAX_NODES = 256    # nodes of one sequence's draft tree
+
+
+def tree_masks(parents) -> tuple[np.ndarray, np.ndarray]:
+    """Ancestor masks and depths of draft trees.  ``parents``: per sequence the
+    parent of every node in node order (-1 for node 0, the root; an earlier
+    node for the others).  Returns the mask rows of all sequences one after
+    another, int64 ``[rows, words]`` (bit ``j % 64`` of word ``j // 64``: node
+    j is the node itself or an ancestor), and the nodes' depths ``[rows]``."""
+    rows = sum(len(p) for p in parents)
+    words = max(1, -(-max((len(p) for p in parents), default=0) // 64))
+    if words * 64 > TREE_MAX_NODES:
+        raise ValueError(f"a draft tree has at most {TREE_MAX_NODES} nodes")
+    mask = np.zeros((rows, words), dtype=np.uint64)
+    depth = np.zeros(rows, dtype=np.int32)
+    r0 = 0
+    for par in parents:
+        for i, p in enumerate(par):
+            if (p != -1) if i == 0 else not 0 <= p < i:
+                raise ValueError(f"node {i}: parent {p} (the root's is -1, others' an earlier node)")
+            if i:
+                mask[r0 + i] = mask[r0 + p]
+                depth[r0 + i] = depth[r0 + p] + 1
+            mask[r0 + i, i >> 6] |= np.uint64(1 << (i & 63))
+        r0 += len(par)
+    return mask.view(np.int64), depth
+
+
 class StepMeta:
     """Device int32 metadata of one flat mixed batch, built on the host with
     numpy and shipped in one host->device copy.  Block tables may be lists
@@ -271,8 +299,12 @@ class StepMeta:
     def __init__(self, token_ids, positions, seq_slices, block_tables, context_lens,
                  block_size: int, group: int, device, pinned: bool = True,
                  all_logits: bool = False, bt_width: int = 0,
-                 dest: torch.Tensor | None = None, staging: torch.Tensor | None = None):
-        """``bt_width`` pads the block tables to at least that many columns
+                 dest: torch.Tensor | None = None, staging: torch.Tensor | None = None,
+                 trees: np.ndarray | None = None):
+        """``trees``: every sequence is a draft tree with these mask rows
+        (``tree_masks``): its tokens go to consecutive slots behind the
+        context before them, whatever their positions, and attention is
+        ``ops.paged_attention_tree``.  ``bt_width`` pads the block tables to at least that many columns
         (a fixed layout for CUDA-graph replay); ``dest``, a device int32
         buffer of exactly the packed size, receives the metadata instead of
         a fresh allocation; ``staging``, a pinned int32 host buffer at least
@@ -307,6 +339,8 @@ class StepMeta:
             first_of_seq = np.repeat(np.cumsum(qlen) - qlen, qlen)
             tok = np.arange(n_tok) - first_of_seq + np.repeat(starts, qlen)
             p = pos[tok].astype(np.int64)
+            if trees is not None:       # siblings share a position, never a slot
+                p = np.repeat(ctx.astype(np.int64) - qlen, qlen) + np.arange(n_tok) - first_of_seq
             blk = p // block_size
             if np.any(blk >= lens[tok_seq]) or np.any(p < 0):
                 raise IndexError("a token position lies beyond its sequence's block table")
@@ -318,6 +352,10 @@ class StepMeta:
             row_dst[ends[qlen > 0] - 1] = np.nonzero(qlen > 0)[0].astype(np.int32)
         self.n_out = T if all_logits else n
         is_dec = qlen * group <= 16
+        is_tree = np.full(n, trees is not None)
+        is_dec &= ~is_tree
+        if trees is not None and trees.shape[0] != T:
+            raise ValueError("one mask row per token")
         self.T, self.n = T, n
         self.group = group
 
@@ -333,12 +371,16 @@ class StepMeta:
             return idx, starts[idx], qlen[idx], ctx[idx], bt
 
         d_idx, d_qs, d_ql, d_ctx, d_bt = subset(is_dec)
-        p_idx, p_qs, p_ql, p_ctx, p_bt = subset(~is_dec)
+        p_idx, p_qs, p_ql, p_ctx, p_bt = subset(~is_dec & ~is_tree)
         work = prefill_work(p_ql, p_ctx, group)
         # decode sequences longest first: the attention grid dispatches in this order
         d_order = np.argsort(-d_ctx, kind="stable").astype(np.int32)
         parts = [ids, pos, slots, row_dst, d_qs, d_ql, d_ctx, d_bt.ravel(), d_order, p_qs, p_ql,
                  p_ctx, p_bt.ravel(), work.ravel()]
+        if trees is not None:       # the 8-byte mask words first, at the buffer's start
+            _, t_qs, t_ql, t_ctx, t_bt = subset(is_tree)
+            words = np.ascontiguousarray(trees, dtype=np.int64).view(np.int32)
+            parts = [words.ravel()] + parts + [t_qs, t_ql, t_ctx, t_bt.ravel()]
         flat = np.concatenate(parts).astype(np.int32)
         if staging is not None and staging.numel() >= flat.size:
             host = staging[: flat.size]
@@ -362,6 +404,17 @@ class StepMeta:
         for a in parts:
             views.append(buf[o:o + a.size])
             o += a.size
+        self.n_tree = 0
+        if trees is not None:
+            mk, *views, tqs, tql, tctx, tbt = views
+            self.n_tree = n
+            self.tree_mask = mk.view(torch.int64).view(T, -1)
+            self.tree_q_start, self.tree_q_len, self.tree_ctx = tqs, tql, tctx
+            self.tree_bt = tbt.view(n, t_bt.shape[1])
+            self.tree_max_q = int(qlen.max()) if n else 0
+            self.tree_max_ctx = int(ctx.max()) if n else 0
+            self.tree_ctx_sum = int(ctx.astype(np.int64).sum())
+            self.tree_pairs = int((qlen.astype(np.int64) * ctx).sum())
         (self.ids, self.positions, self.slots, self.row_dst, self.dec_q_start, self.dec_q_len,
          self.dec_ctx, dbt, self.dec_order, self.pre_q_start, self.pre_q_len, self.pre_ctx, pbt,
          wk) = views
@@ -548,6 +601,14 @@ class DeviceModel:
                     4.0 * md.pre_pairs * W.n_q * hd, ops.paged_attention_prefill,
                     self.q, self.attn, pool, block_tables=md.pre_bt, q_start=md.pre_q_start,
                     q_len=md.pre_q_len, ctx_len=md.pre_ctx, work=md.work, **akw)
+            if md.n_tree:
+                self._run(
+                    "attention_tree", md.tree_ctx_sum * kv_row + 2 * T * qrow,
+                    4.0 * md.tree_pairs * W.n_q * hd, ops.paged_attention_tree,
+                    self.q[:T], self.attn[:T], pool, block_tables=md.tree_bt,
+                    q_start=md.tree_q_start, q_len=md.tree_q_len, ctx_len=md.tree_ctx,
+                    tree_mask=md.tree_mask, max_q=md.tree_max_q, max_ctx=md.tree_max_ctx,
+                    ctx_total=md.tree_ctx_sum, **akw)
             parts = self._row(self.attn[:T], L.wo, L.ln_post, T, False, md, 2 * li, pl["o"])
             bn, splits = pl["gu"]
             Ngu = L.wgu.shape[0]
