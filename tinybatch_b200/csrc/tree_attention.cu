@@ -143,6 +143,554 @@ static int tree_simple_launch(const TreeAttnArgs& t, cudaStream_t st) {
                     dim3(TS_WARPS * 32), 0, st, 1, "tree attention launch", t);
 }
 
+// -------------------------------------------------------------- tensor cores
+//
+// One CTA per (row tile of 128 query rows, kv head, sequence) and split of its
+// context; the splits of a row tile form a cluster of C CTAs (1 to 8).  S = Q K^T and O += P V
+// run on tcgen05 (M = 128 rows, tiles of 64 keys) with S, P and O in TMEM:
+//   warps 0-3  softmax: one query row a thread (TMEM lane = row); warps whose
+//              rows do not exist stay out
+//   warp 4     TMA: every 16 tokens one box {64 columns, 8 tokens, halves, K/V,
+//              2} of a 5-d view of the pool, i.e. K and V of a block and head in
+//              one request (8 KiB at hd 128).  It lands as [8-token group][K, V]
+//              [half][8][128 B], 128-byte swizzled, so K is a K-major operand and
+//              V an MN-major one whose 8-token groups lie 2 * halves KiB apart
+//   warp 5     MMA issue: S of the next tile goes into the other S buffer while
+//              the softmax works on this one; P (bf16) overwrites S in place and
+//              is read from TMEM
+// O is accumulated in TMEM; a row's exponent reference moves only when its
+// maximum has grown by more than TT_RESCALE (log2 units), as in the prefill kernel.
+// A quarter of an SM's shared memory would hold fewer keys in flight than HBM's
+// latency asks for, half of it with two CTAs an SM hides one CTA's chain S ->
+// softmax -> P V, its start and its end behind the other's loads.
+//
+// Tiles that hold drafts (or places past the context) apply the mask to S and
+// clean V in shared memory before P V: rows past the context become zero (a
+// block's rest may hold anything, and 0 * NaN is NaN), and so do non-finite
+// elements of draft nodes, which the epilogue adds back to the rows that see
+// them.
+//
+// With C > 1 every CTA leaves (reference, sum, O) of its rows in its own shared
+// memory and each merges 1/C of the rows over the cluster, in split order: no
+// workspace, no counters, nothing shared between calls.
+constexpr int TT_ROWS = 128;
+constexpr int TT_KEYS = 64;
+constexpr int TT_THREADS = 192;
+constexpr float TT_RESCALE = 8.f;
+constexpr int TT_MAX_SPLITS = 8;
+
+template <int HD>
+struct TreeTcLayout {
+  static constexpr int HALVES = HD / 64;
+  static constexpr int Q_HALF = TT_ROWS * 128;
+  static constexpr int Q_TILE = HALVES * Q_HALF;
+  static constexpr int GROUP = 2 * HALVES * 1024;      // 8 tokens: K halves, V halves
+  static constexpr int BOX = 2 * GROUP;                // 16 tokens
+  static constexpr int STAGE = TT_KEYS / 16 * BOX;
+  static constexpr int STAGES = HD == 128 ? 2 : 4;
+  static constexpr int OFF_KV = Q_TILE;
+  static constexpr int LDO = HD + 4;                   // floats a merged row (conflict-free float4 rows)
+  static constexpr int OFF_ML = OFF_KV + STAGES * STAGE;
+  static constexpr int OFF_BAR = OFF_ML + TT_ROWS * 8;
+  static constexpr int N_BARS = 2 * STAGES + 7;
+  static constexpr int SMEM = OFF_BAR + 32 * 8 + 1024;
+  static constexpr uint32_t COL_O = 2 * TT_KEYS;
+  static constexpr uint32_t TMEM_COLS = 256;
+  static_assert(TT_ROWS * LDO * 4 <= OFF_ML, "merge rows over Q and the ring");
+  static_assert(N_BARS * 8 + 8 <= 32 * 8, "barrier area");
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
+  static_assert(2 * TT_KEYS + HD <= 256, "TMEM: two S buffers and O in half of it");
+};
+
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int x4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %3, %3, %3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(x4)
+      : "memory");
+}
+
+// K-major 128-byte-swizzled operand whose 8-row atoms lie sbo bytes apart.
+__device__ __forceinline__ uint64_t sw128_k_desc(uint32_t smem_addr, uint32_t sbo) {
+  return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(sbo >> 4) << 32 |
+         (uint64_t)1u << 46 | (uint64_t)2u << 61;
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// Bits of a word whose bf16 halves are infinite or NaN (those halves all ones).
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
+  return ((w & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u) |
+         ((w & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u);
+}
+
+// Which of the keys k0 .. k0+63 a row sees (base: first draft's position).
+__device__ __forceinline__ unsigned long long tree_window(const unsigned long long* m, int k0,
+                                                          int base, int ctx) {
+  const int d = k0 - base;
+  unsigned long long w;
+  if (d <= -64) {
+    w = ~0ull;
+  } else if (d < 0) {
+    w = ((1ull << -d) - 1) | (m[0] << -d);
+  } else {
+    const int k = d >> 6, o = d & 63;
+    unsigned long long lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < TREE_WORDS; ++i) {
+      if (i == k) lo = m[i];
+      if (i == k + 1) hi = m[i];
+    }
+    w = o ? (lo >> o) | (hi << (64 - o)) : lo;
+  }
+  const int left = ctx - k0;
+  if (left < 64) w &= left > 0 ? (1ull << left) - 1 : 0ull;
+  return w;
+}
+
+// For every non-finite value of the draft nodes j0 .. j1-1 that row `row` sees
+// (their products were left out of P V): add(column, value).
+template <int HD, class F>
+__device__ __forceinline__ void for_nonfinite(const TreeAttnArgs& t, const int* table, int kvh,
+                                              size_t row, int base, int j0, int j1, F add) {
+  const AttnArgs& a = t.a;
+#pragma unroll 1
+  for (int j = j0; j < j1; ++j) {
+    if (!((t.mask[row * t.mask_ld + (j >> 6)] >> (j & 63)) & 1)) continue;
+    const int p = base + j;
+    const int blk = table[p / a.block_size];
+    if (blk < 0 || blk >= a.num_blocks) continue;
+    const __nv_bfloat16* src =
+        a.pool + (((size_t)blk * 2 + 1) * a.n_kv_heads + kvh) * a.block_size * HD +
+        (size_t)(p % a.block_size) * HD;
+#pragma unroll 1
+    for (int c = 0; c < HD; ++c) {
+      const float x = __bfloat162float(src[c]);
+      if (!isfinite(x)) add(c, x);
+    }
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(TT_THREADS, 2)
+    tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map, const TreeAttnArgs t,
+                        const int row_tiles) {
+  using L = TreeTcLayout<HD>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = align_smem_1024(smem_raw);
+  float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);   // [STAGES]
+  uint64_t* empty = full + L::STAGES;                               // [STAGES]
+  uint64_t* s_full = empty + L::STAGES;                             // [2]
+  uint64_t* p_full = s_full + 2;                                    // [2]
+  uint64_t* pv_done = p_full + 2;                                   // [2]
+  uint64_t* q_full = pv_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
+  int* s_bad = reinterpret_cast<int*>(tmem_slot + 1);   // a draft's V has non-finite elements
+
+  const AttnArgs& a = t.a;
+  const int C = gridDim.x, rank = blockIdx.x;     // cluster = (C, 1, 1)
+  const int kvh = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles;
+  const int seq = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, L::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) prefetch_tmap(&map);
+  pdl_wait();
+  TreeSeq s;
+  const bool ok = tree_seq(t, seq, s);
+  const int G = a.n_q_heads / a.n_kv_heads;
+  const int rows = s.ql * G - rt * TT_ROWS;        // of this tile on
+  if (!ok || rows <= 0) {                          // uniform over the cluster
+    if (!ok && rt == 0 && threadIdx.x == 0) set_status(ERR_BAD_INDEX);
+    __syncthreads();
+    if (warp == 5) tmem_dealloc(*tmem_slot, L::TMEM_COLS);
+    return;
+  }
+  const int nrows = min(rows, TT_ROWS);
+  const int act = (nrows + 31) / 32;               // softmax warps with rows
+  const int* table = a.block_tables + (size_t)seq * a.bt_ld;
+  const int n_chunks = (s.ctx + 15) / 16;
+  const int tiles = (s.ctx + TT_KEYS - 1) / TT_KEYS;
+  const int t0 = (int)((long long)tiles * rank / C);
+  const int nt = (int)((long long)tiles * (rank + 1) / C) - t0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 32 * act);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(q_full, 32 * act);
+    *s_bad = 0;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // only now: a dependent kernel that takes tensor memory must not get in before this CTA's
+  if (threadIdx.x == 0) pdl_trigger();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t sbase = smem_u32(smem);
+  float ref = -INFINITY, l = 0.f;                  // a row's exponent reference (log2) and sum
+  unsigned long long m[TREE_WORDS] = {0, 0, 0, 0};
+
+  if (warp == 4) {
+    // ---------------- loader
+    int ids = 0;
+    for (int j = 0; j < nt; ++j) {
+      const int st = j % L::STAGES;
+      const int c0 = (t0 + j) * (TT_KEYS / 16);
+      if (j % 8 == 0) {      // lane i: block of chunk c0 + i, for eight tiles
+        const int c = c0 + lane;
+        if (c < n_chunks) {
+          ids = table[c * 16 / a.block_size];
+          if (ids < 0 || ids >= a.num_blocks) {
+            set_status(ERR_BAD_INDEX);
+            ids = 0;         // load something valid; the result is flagged
+          }
+        }
+      }
+      if (j >= L::STAGES &&
+          !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / L::STAGES) - 1) & 1)))
+        break;
+      const int nb = min(TT_KEYS / 16, n_chunks - c0);
+      const int blk = __shfl_sync(0xffffffffu, ids, ((j % 8) * 4 + lane) & 31);
+      if (lane == 0) mbar_arrive_expect_tx(&full[st], nb * L::BOX);
+      __syncwarp();
+      if (lane < nb) {
+        const int slot = (c0 + lane) * 16 % a.block_size;
+        tma_load_5d(smem + L::OFF_KV + st * L::STAGE + lane * L::BOX, &map, &full[st],
+                    ((blk * 2 * a.n_kv_heads + kvh) * a.block_size + slot) / 8);
+      }
+    }
+  } else if (warp == 5) {
+    // ---------------- MMA issue
+    if (lane == 0 && nt > 0) {
+      constexpr uint32_t idesc_s = idesc_bf16_m128(TT_KEYS);
+      constexpr uint32_t idesc_o = idesc_bf16_m128(HD) | (1u << 16);   // V: MN-major
+      auto issue_s = [&](int j) -> bool {
+        const int st = j % L::STAGES;
+        if (!mbar_wait(&full[st], (j / L::STAGES) & 1)) return false;
+        tc_fence_after();
+        const uint32_t kb = sbase + L::OFF_KV + st * L::STAGE;
+#pragma unroll
+        for (int h = 0; h < L::HALVES; ++h)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_bf16(tmem + (j & 1) * TT_KEYS, sw128_desc(sbase + h * L::Q_HALF + kk * 32),
+                        sw128_k_desc(kb + h * 1024 + kk * 32, L::GROUP), idesc_s,
+                        (h | kk) ? 1u : 0u);
+        tc_commit(&s_full[j & 1]);
+        return true;
+      };
+      bool good = mbar_wait(q_full, 0);
+      tc_fence_after();
+      if (good) good = issue_s(0);
+      for (int j = 0; j < nt && good; ++j) {
+        if (j + 1 < nt) {
+          // S of the next tile overwrites P of the previous one
+          if (j > 0) good = mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);
+          if (good) good = issue_s(j + 1);
+          if (!good) break;
+        }
+        if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1)) break;
+        tc_fence_after();
+        const int st = j % L::STAGES;
+        const uint32_t vb = sbase + L::OFF_KV + st * L::STAGE + L::HALVES * 1024;
+#pragma unroll
+        for (int ks = 0; ks < TT_KEYS / 16; ++ks)
+          tc_mma_bf16_ts(tmem + L::COL_O, tmem + (j & 1) * TT_KEYS + ks * 8,
+                         sw128_mn_desc(vb + ks * 2 * L::GROUP, 1024, L::GROUP), idesc_o,
+                         (j | ks) ? 1u : 0u);
+        tc_commit(&empty[st]);
+        tc_commit(&pv_done[j & 1]);
+      }
+    }
+    __syncwarp();
+  } else if (warp < act) {
+    // ---------------- softmax: one row a thread
+    const int r = threadIdx.x;
+    const bool valid = r < nrows;
+    const int R = rt * TT_ROWS + (valid ? r : 0);
+    const size_t row = (size_t)s.q0 + R / G;
+#pragma unroll
+    for (int i = 0; i < TREE_WORDS; ++i)
+      if (i < t.mask_w && valid) m[i] = t.mask[row * t.mask_ld + i];
+    {
+      // the warp's 32 rows, HD/8 lanes a row; missing rows are zero
+      constexpr int PPR = HD / 8, RPI = 32 / PPR;
+      const unsigned long long mine =
+          valid ? row * a.ld_q + (size_t)(kvh * G + R % G) * HD : ~0ull;
+      uint4 v[32 / RPI];
+#pragma unroll
+      for (int i = 0; i < 32 / RPI; ++i) {
+        const unsigned long long off = __shfl_sync(0xffffffffu, mine, i * RPI + lane / PPR);
+        v[i] = off != ~0ull ? *reinterpret_cast<const uint4*>(a.q + off + (lane % PPR) * 8)
+                            : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < 32 / RPI; ++i) {
+        const int c = lane % PPR;
+        *reinterpret_cast<uint4*>(smem + (c >> 3) * L::Q_HALF +
+                                  sw128_off(warp * 32 + i * RPI + lane / PPR, c & 7)) = v[i];
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+    }
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    const uint32_t to = tmem + L::COL_O + lane_off;
+    const float sc = a.scale_log2;
+    int done = 0;
+    for (int j = 0; j < nt; ++j) {
+      const int k0 = (t0 + j) * TT_KEYS;
+      const uint32_t ts = tmem + (j & 1) * TT_KEYS + lane_off;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], (j >> 1) & 1))) break;
+      tc_fence_after();
+      float x[TT_KEYS];
+      tmem_ld64(ts, x);
+      if (k0 + TT_KEYS > s.base) {                 // drafts, or places past the context
+        const unsigned long long w = tree_window(m, k0, s.base, s.ctx);
+        const uint32_t wl = (uint32_t)w, wh = (uint32_t)(w >> 32);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          if (!(wl & (1u << e))) x[e] = -INFINITY;
+          if (!(wh & (1u << e))) x[32 + e] = -INFINITY;
+        }
+        const int st = j % L::STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (j / L::STAGES) & 1))) break;
+        uint8_t* vb = smem + L::OFF_KV + st * L::STAGE + L::HALVES * 1024;
+        const int first = max(s.base - k0, 0);
+        for (int i = first * (HD / 8) + r; i < TT_KEYS * (HD / 8); i += 32 * act) {
+          const int key = i / (HD / 8), c = i % (HD / 8);
+          uint4* p = reinterpret_cast<uint4*>(vb + (key >> 3) * L::GROUP + (c >> 3) * 1024 +
+                                              sw128_off(key & 7, c & 7));
+          if (k0 + key >= s.ctx) {
+            *p = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            uint4 q = *p;
+            const uint4 n = make_uint4(nonfinite2(q.x), nonfinite2(q.y), nonfinite2(q.z), nonfinite2(q.w));
+            if (n.x | n.y | n.z | n.w) {
+              q.x &= ~n.x, q.y &= ~n.y, q.z &= ~n.z, q.w &= ~n.w;
+              *p = q;
+              *s_bad = 1;
+            }
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < TT_KEYS; e += 2) mx = fmax3(mx, x[e], x[e + 1]);
+      mx *= sc;
+      const bool move = mx > ref + TT_RESCALE;     // any finite max when ref is -inf
+      const bool rescale = move && ref != -INFINITY;
+      const float alpha = rescale ? ex2_approx(ref - mx) : 1.f;
+      if (__any_sync(0xffffffffu, rescale)) {
+        // O holds the tiles before this one: once the last of them is in, scale it
+        if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c0 = 0; c0 < HD; c0 += 32) {
+          float v[32];
+          tmem_ld32(to + c0, v);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] *= alpha;
+          tmem_st32(to + c0, v);
+        }
+      }
+      if (move) ref = mx;
+      l *= alpha;
+      const float mu = ref == -INFINITY ? 0.f : ref;
+      const float2 sc2 = make_float2(sc, sc), nmu2 = make_float2(-mu, -mu);
+      float2 sum2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c0 = 0; c0 < TT_KEYS; c0 += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 xv = fma2(make_float2(x[c0 + e], x[c0 + e + 1]), sc2, nmu2);
+          const float2 pv = make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
+          sum2 = add2(sum2, pv);
+          w[e >> 1] = pack_bf16x2(pv.x, pv.y);
+        }
+        tmem_st16(ts + (c0 >> 1), w);
+      }
+      tmem_wait_st();
+      l += sum2.x + sum2.y;
+      tc_fence_before();
+      mbar_arrive(&p_full[j & 1]);
+      done = j + 1;
+    }
+    if (nt > 0 && done == nt) {
+      __all_sync(0xffffffffu, mbar_wait(&pv_done[(nt - 1) & 1], ((nt - 1) >> 1) & 1));
+      tc_fence_after();
+    }
+  }
+  __syncthreads();      // every load has landed and every MMA is complete
+
+  // ---------------- epilogue
+  const int j0 = max(t0 * TT_KEYS - s.base, 0);                        // this split's draft nodes
+  const int j1 = min((t0 + nt) * TT_KEYS - s.base, s.ql);
+  const bool bad = *s_bad != 0;
+  if (warp < act) {
+    const int r = threadIdx.x;
+    const bool valid = r < nrows;
+    const int R = rt * TT_ROWS + (valid ? r : 0);
+    const uint32_t to = tmem + L::COL_O + ((uint32_t)(warp * 32) << 16);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    __nv_bfloat16* dst =
+        a.out + ((size_t)s.q0 + R / G) * a.ld_out + (size_t)(kvh * G + R % G) * HD;
+    float* keep = reinterpret_cast<float*>(smem) + r * L::LDO;
+#pragma unroll
+    for (int c0 = 0; c0 < HD; c0 += 32) {
+      float v[32];
+      if (nt > 0) {
+        tmem_ld32(to + c0, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0.f;
+      }
+      if (C > 1) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<float4*>(keep + c0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+      } else if (valid) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = l == 0.f ? 0.f : v[e] * inv;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) store_bf16x8(dst + c0 + e, v + e);
+      }
+    }
+    if (C > 1) s_ml[r] = make_float2(ref, l);
+    if (bad && valid)
+      for_nonfinite<HD>(t, table, kvh, (size_t)s.q0 + R / G, s.base, j0, j1, [&](int c, float x) {
+        if (C > 1) keep[c] += x;
+        else dst[c] = __float2bfloat16_rn(__bfloat162float(dst[c]) + x);
+      });
+  }
+  tc_fence_before();
+  if (C == 1) {
+    __syncthreads();
+  } else {
+    cluster_sync_all();
+    // this CTA's 1/C of the rows: HD/4 lanes a row, four columns each
+    constexpr int LPR = HD / 4, RPW = 32 / LPR;
+    const int per = (nrows + C - 1) / C;
+    const int r1 = min((rank + 1) * per, nrows);
+    for (int rb = rank * per + warp * RPW; rb < r1; rb += (TT_THREADS / 32) * RPW) {
+      const int r = rb + lane / LPR;
+      const int rr = min(r, r1 - 1);
+      const int c = (lane % LPR) * 4;
+      float2 ml[TT_MAX_SPLITS];
+      float M = -INFINITY;
+#pragma unroll
+      for (int z = 0; z < TT_MAX_SPLITS; ++z)
+        if (z < C) {
+          ml[z] = ld_cluster_f2(cluster_map(sbase + L::OFF_ML + rr * 8, z));
+          M = fmaxf(M, ml[z].x);
+        }
+      const float mu = M == -INFINITY ? 0.f : M;
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int z = 0; z < TT_MAX_SPLITS; ++z)
+        if (z < C && !(ml[z].x == -INFINITY && ml[z].y == 0.f)) {   // a split that saw nothing
+          const float w = ex2_approx(ml[z].x - mu);
+          const float4 o = ld_cluster_f4(cluster_map(sbase + (rr * L::LDO + c) * 4, z));
+          sum += w * ml[z].y;
+          acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
+        }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      if (r < r1) {
+        const int R = rt * TT_ROWS + r;
+        uint2 u;
+        u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+        u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>(a.out + ((size_t)s.q0 + R / G) * a.ld_out +
+                                  (size_t)(kvh * G + R % G) * HD + c) = u;
+      }
+    }
+    cluster_sync_all();   // peers read this CTA's shared memory until here
+  }
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::TMEM_COLS);
+  }
+}
+
+// The pool as {64 columns, 8 tokens, halves, K/V, 8-token groups}: group g of
+// (block, K, head) starts at ((block * 2) * n_kv + head) * bs / 8 + g, its V one
+// K/V stride further.
+template <int HD>
+static int tree_pool_map(CUtensorMap* map, const AttnArgs& a) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_last_error("cuTensorMapEncodeTiled entry point unavailable");
+    return TB_ERR_CUDA;
+  }
+  const cuuint64_t per_kv = (cuuint64_t)a.n_kv_heads * a.block_size;   // tokens between K and V
+  const cuuint64_t dims[5] = {64, 8, HD / 64, 2, ((cuuint64_t)a.num_blocks * 2 - 1) * per_kv / 8};
+  const cuuint64_t strides[4] = {HD * 2, 128, per_kv * HD * 2, 8 * HD * 2};
+  const cuuint32_t box[5] = {64, 8, HD / 64, 2, 2};
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<__nv_bfloat16*>(a.pool),
+                        dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_last_error("cuTensorMapEncodeTiled failed (%d) for the KV pool", (int)r);
+    return TB_ERR_CUDA;
+  }
+  return TB_OK;
+}
+
+// CTAs that share a context: as many as let the longest context's share be no
+// longer than the average work of a resident CTA (148 SMs x 2), so that one wave covers a
+// small batch and a long context does not outlast the others, but no share
+// below four tiles (the merge costs more than it saves).
+static int tree_splits(int n_seqs, int n_kv, int row_tiles, int max_ctx, long long ctx_total) {
+  const long long share = ctx_total * n_kv * row_tiles / (148 * 2);
+  const long long least = 4 * TT_KEYS;
+  const long long c = max_ctx / (share > least ? share : least);
+  return c >= 8 ? 8 : c >= 4 ? 4 : c >= 2 ? 2 : 1;
+}
+
+template <int HD>
+static int tree_tc_launch(const TreeAttnArgs& t, int max_ctx, long long ctx_total, cudaStream_t st) {
+  using L = TreeTcLayout<HD>;
+  static std::atomic<unsigned long long> attr_devs{0};
+  if (int rc = smem_attr_once(tree_attn_tc_kernel<HD>, L::SMEM, attr_devs,
+                              "tree attention smem attribute", true))
+    return rc;
+  CUtensorMap map;
+  if (int rc = tree_pool_map<HD>(&map, t.a)) return rc;
+  const long long rows = (long long)t.max_q * (t.a.n_q_heads / t.a.n_kv_heads);
+  const int row_tiles = (int)((rows + TT_ROWS - 1) / TT_ROWS);
+  if ((long long)row_tiles * t.a.n_kv_heads > 65535) return arg_err("too many heads and nodes");
+  const int C = tree_splits(t.a.n_seqs, t.a.n_kv_heads, row_tiles, max_ctx, ctx_total);
+  return launch_pdl(tree_attn_tc_kernel<HD>, dim3(C, t.a.n_kv_heads * row_tiles, t.a.n_seqs),
+                    dim3(TT_THREADS), L::SMEM, st, C, "tree attention launch", map, t, row_tiles);
+}
+
 int tree_attention(TreeAttnArgs t, int head_dim, int max_ctx, long long ctx_total,
                    cudaStream_t st) {
   AttnArgs& a = t.a;
@@ -168,10 +716,17 @@ int tree_attention(TreeAttnArgs t, int head_dim, int max_ctx, long long ctx_tota
   for (const void* p : {(const void*)a.q, (const void*)a.out, (const void*)a.pool})
     if (reinterpret_cast<uintptr_t>(p) % 16) return arg_err("q / out / kv_pool must be 16-byte aligned");
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
+  const long long width = (long long)t.bt_w * a.block_size;   // tokens a table row can hold
+  if (max_ctx <= 0 || max_ctx > width) max_ctx = (int)(width < 0x7fffffff ? width : 0x7fffffff);
+  if (ctx_total <= 0 || ctx_total > (long long)max_ctx * a.n_seqs)
+    ctx_total = (long long)max_ctx * a.n_seqs;
+  // 16-token boxes inside one block; the group index is a 32-bit coordinate
+  const bool tc = a.block_size % 16 == 0 &&
+                  (long long)a.num_blocks * 2 * a.n_kv_heads * a.block_size < (1ll << 31);
   switch (head_dim) {
     case 16: return tree_simple_launch<16>(t, st);
-    case 64: return tree_simple_launch<64>(t, st);
-    default: return tree_simple_launch<128>(t, st);
+    case 64: return tc ? tree_tc_launch<64>(t, max_ctx, ctx_total, st) : tree_simple_launch<64>(t, st);
+    default: return tc ? tree_tc_launch<128>(t, max_ctx, ctx_total, st) : tree_simple_launch<128>(t, st);
   }
 }
 
