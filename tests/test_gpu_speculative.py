@@ -312,6 +312,8 @@ def test_tree_attention_refuses_arguments():
         c.run(dict(d, bt=d["bt"].cpu()))
     with pytest.raises(ValueError, match="kv_pool"):
         c.run(dict(d, pool=d["pool"][..., :32]))
+    with pytest.raises(ValueError, match="columns"):
+        c.run(dict(d, q=d["q"][:, :192]))
     with pytest.raises(ValueError, match="contiguous"):
         c.run(dict(d, pool=d["pool"][::2]))
     with pytest.raises(_native.NativeError, match="max_q"):

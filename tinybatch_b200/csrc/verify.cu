@@ -33,9 +33,10 @@
 namespace tb {
 
 constexpr int VF_NODES = 256;      // nodes of a sequence's tree
-constexpr int VF_THREADS = 512;
-constexpr int VF_WARPS = VF_THREADS / 32;
-constexpr int VF_MAX_CLUSTER = 8;
+constexpr int VF_MAX_WARPS = 16;
+constexpr int VF_MAX_CLUSTER = 16;
+constexpr int VF_GROUPS = 4;       // 128-token groups whose loads a warp has in flight
+constexpr int VF_BATCHES = 32;     // sums a warp keeps of its part of the vocabulary
 
 struct TreeArgs {
   const int *ids, *parents, *q_start, *q_len;
@@ -127,22 +128,17 @@ struct Rejections {
   double inv_z[VF_NODES];     // 1 / Z, or 0 where Z was 0 (r kept)
 };
 
-// r after every rejection of h at a token with target probability p and draft
-// probability d; `special`: the token is among the rejected ones.
-template <bool DIST>
-__device__ __forceinline__ double residual(const Rejections& h, int token, float p, float d,
-                                           bool special) {
-  double r = p;
-  if (DIST) {
-    double dd = d;
-    for (int k = 0; k < h.n; ++k) {
-      const double iz = h.inv_z[k];
-      if (iz > 0.0) r = fmax(r - dd * h.scale[k], 0.0) * iz;
-      if (special && h.token[k] == token) dd = 0.0;
+// r of one token with target probability p and draft probability d after
+// every rejection of h.
+__device__ __forceinline__ double residual(const Rejections& h, bool dist, int token, float p,
+                                           float d) {
+  double r = p, dd = d;
+  for (int k = 0; k < h.n; ++k) {
+    if (dist && h.inv_z[k] > 0.0) r = fmax(r - dd * h.scale[k], 0.0) * h.inv_z[k];
+    if (h.token[k] == token) {
+      if (dist) dd = 0.0;
+      else r = 0.0;
     }
-  } else if (special) {
-    for (int k = 0; k < h.n; ++k)
-      if (h.token[k] == token) r = 0.0;
   }
   return r;
 }
@@ -153,42 +149,81 @@ __device__ __forceinline__ bool rejected(const Rejections& h, int first, int cou
   return s;
 }
 
-// r of the four consecutive tokens from y on (0 from `end` on).
-template <bool DIST>
-__device__ __forceinline__ void residual4(const Rejections& h, const float* p, const float* d,
-                                          int y, int end, bool vec, double* w) {
-  float pv[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
-  if (vec && y + 4 <= end) {
-    const float4 a = *reinterpret_cast<const float4*>(p + y);
-    pv[0] = a.x, pv[1] = a.y, pv[2] = a.z, pv[3] = a.w;
-    if (DIST) {
-      const float4 b = *reinterpret_cast<const float4*>(d + y);
-      dv[0] = b.x, dv[1] = b.y, dv[2] = b.z, dv[3] = b.w;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (y + e < end) {
-        pv[e] = p[y + e];
-        if (DIST) dv[e] = d[y + e];
-      }
-  }
-  const bool special = rejected(h, y, 4);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = residual<DIST>(h, y + e, pv[e], dv[e], special);
+__device__ __forceinline__ float4 load4(const float* row, int y, int end, bool vec) {
+  if (vec && y + 4 <= end) return __ldg(reinterpret_cast<const float4*>(row + y));
+  return make_float4(y < end ? __ldg(row + y) : 0.f, y + 1 < end ? __ldg(row + y + 1) : 0.f,
+                     y + 2 < end ? __ldg(row + y + 2) : 0.f, y + 3 < end ? __ldg(row + y + 3) : 0.f);
 }
 
-// One cluster a sequence, the vocabulary cut into one segment a warp.  Every
-// CTA walks the tree alike (same loads, same arithmetic), so the cluster only
-// meets for sums over the vocabulary: one after each rejection that has to
-// know Z, one for the sample.
-__global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) {
+// r of tokens y + 128 g .. + 3, g < VF_GROUPS (y already the lane's; 0 from
+// `end` on).  All loads are issued before the first is used.
+template <bool DIST>
+__device__ __forceinline__ void weights(const Rejections& h, const float* p, const float* d, int y,
+                                        int end, bool vec, double (*w)[4]) {
+  float4 pv[VF_GROUPS], dv[VF_GROUPS];
+#pragma unroll
+  for (int g = 0; g < VF_GROUPS; ++g) pv[g] = load4(p, y + 128 * g, end, vec);
+  if (DIST)
+#pragma unroll
+    for (int g = 0; g < VF_GROUPS; ++g) dv[g] = load4(d, y + 128 * g, end, vec);
+#pragma unroll
+  for (int g = 0; g < VF_GROUPS; ++g)
+    w[g][0] = pv[g].x, w[g][1] = pv[g].y, w[g][2] = pv[g].z, w[g][3] = pv[g].w;
+  // the warp's stretch holds a rejected token (rare): only then are tokens compared
+  const bool special = rejected(h, y & ~127, 128 * VF_GROUPS);
+  for (int k = 0; k < h.n; ++k) {
+    if (DIST) {
+      const double sc = h.scale[k], iz = h.inv_z[k];
+      if (iz > 0.0) {
+#pragma unroll
+        for (int g = 0; g < VF_GROUPS; ++g) {
+          w[g][0] = fmax(w[g][0] - dv[g].x * sc, 0.0);
+          w[g][1] = fmax(w[g][1] - dv[g].y * sc, 0.0);
+          w[g][2] = fmax(w[g][2] - dv[g].z * sc, 0.0);
+          w[g][3] = fmax(w[g][3] - dv[g].w * sc, 0.0);
+        }
+        if (iz != 1.0)
+#pragma unroll
+          for (int g = 0; g < VF_GROUPS; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[g][e] *= iz;
+      }
+    }
+    if (special) {
+      const int x = h.token[k] - y;
+#pragma unroll
+      for (int g = 0; g < VF_GROUPS; ++g) {
+        if (DIST) {
+          if (x == 128 * g) dv[g].x = 0.f;
+          if (x == 128 * g + 1) dv[g].y = 0.f;
+          if (x == 128 * g + 2) dv[g].z = 0.f;
+          if (x == 128 * g + 3) dv[g].w = 0.f;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (x == 128 * g + e) w[g][e] = 0.0;
+        }
+      }
+    }
+  }
+}
+
+// One cluster a sequence, the vocabulary cut into one segment a warp and a
+// segment into at most VF_BATCHES batches.  Every CTA walks the tree alike (same
+// loads, same arithmetic), so the cluster only meets for sums over the
+// vocabulary: one for each rejection whose Z a later sibling's test needs, one
+// for the sample.
+template <int THREADS, int MIN_CTAS>
+__global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyArgs a) {
   namespace cg = cooperative_groups;
+  constexpr int WARPS = THREADS / 32;
+  static_assert(WARPS <= VF_MAX_WARPS, "sum slots");
   __shared__ int s_id[VF_NODES], s_first[VF_NODES], s_sib[VF_NODES], s_par[VF_NODES];
   __shared__ float s_p[VF_NODES], s_d[VF_NODES], s_u[VF_NODES];
   __shared__ int s_drow[VF_NODES];
   __shared__ Rejections s_h;
-  __shared__ double s_sum[2][VF_MAX_CLUSTER * VF_WARPS];
+  __shared__ double s_sum[2][VF_MAX_CLUSTER * WARPS];
+  __shared__ double s_batch[WARPS][VF_BATCHES];
   __shared__ double s_prefix[VF_MAX_CLUSTER + 1];
   cg::cluster_group cluster = cg::this_cluster();
   pdl_wait();
@@ -203,7 +238,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
   if (!ok || ql == 0) {   // uniform over the cluster
     if (rank == 0) {
       if (!ok && tid == 0) set_status(ERR_BAD_INDEX);
-      for (int k = tid; k < t.path_w; k += VF_THREADS) path[k] = -1;
+      for (int k = tid; k < t.path_w; k += THREADS) path[k] = -1;
       if (tid == 0) {
         t.n_accepted[seq] = 0;
         t.next_ids[seq] = -1;
@@ -211,11 +246,10 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
     }
     return;
   }
-
   auto started = cluster.barrier_arrive();   // waited for before the first remote store
 
   // ---- the tree and, for every node, the probabilities its test compares
-  for (int i = tid; i < ql; i += VF_THREADS) {
+  for (int i = tid; i < ql; i += THREADS) {
     int p = t.parents[q0 + i];
     const int id = t.ids[q0 + i];
     int dr = a.draft_rows != nullptr ? a.draft_rows[q0 + i] : -1;
@@ -237,7 +271,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
     s_p[i] = p >= 0 ? a.probs[(size_t)(q0 + p) * a.ld_p + id] : 0.f;
   }
   __syncthreads();
-  for (int i = tid; i < ql; i += VF_THREADS) {
+  for (int i = tid; i < ql; i += THREADS) {
     const int p = s_par[i];
     int sib = VF_NODES;
     if (p >= 0) {
@@ -256,33 +290,42 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
   __syncthreads();
   cluster.barrier_wait(std::move(started));
 
-  // this warp's segment of the vocabulary
-  const int n_seg = C * VF_WARPS;
-  const int seg_len = ((a.vocab + n_seg * 128 - 1) / (n_seg * 128)) * 128;
-  const int seg = rank * VF_WARPS + warp;
-  const long long y_begin = (long long)seg * seg_len;
-  const int y0 = y_begin < a.vocab ? (int)y_begin : a.vocab;
-  const int y1 = y_begin + seg_len < a.vocab ? (int)(y_begin + seg_len) : a.vocab;
+  // this warp's segment of the vocabulary, in batches
+  const int step = 128 * VF_GROUPS;
+  const int n_seg = C * WARPS;
+  const int batch = ((a.vocab + n_seg * VF_BATCHES - 1) / (n_seg * VF_BATCHES) + step - 1) / step * step;
+  const int n_batch = ((a.vocab + n_seg - 1) / n_seg + batch - 1) / batch;
+  const int seg = rank * WARPS + warp;
+  const long long y_begin = (long long)seg * n_batch * batch;
+  const int y0 = (int)min(y_begin, (long long)a.vocab);
+  const int y1 = (int)min(y_begin + (long long)n_batch * batch, (long long)a.vocab);
   const bool vec_p = a.ld_p % 4 == 0 && reinterpret_cast<uintptr_t>(a.probs) % 16 == 0;
   const bool vec_d = a.ld_d % 4 == 0 && reinterpret_cast<uintptr_t>(a.draft_probs) % 16 == 0;
   int parity = 0;
   double* sums = s_sum[0];
 
   // Sum over the vocabulary of r with the rejections of s_h applied.  All
-  // threads of the cluster call it; every one gets the same sum.  s_prefix:
-  // the CTAs' exclusive prefix sums, summed in rank order (so they never
-  // decrease), and the total.
+  // threads of the cluster call it; every one gets the same sum.  s_batch: the
+  // batches' sums; s_prefix: the CTAs' exclusive prefix sums, summed in rank
+  // order (so they never decrease), and the total.
   auto vocab_sum = [&](const float* p, const float* d, bool dist) -> double {
     double acc = 0.0;
     const bool vec = vec_p && (!dist || vec_d);
-    for (int y = y0 + 4 * lane; y < y1; y += 128) {
-      double w[4];
-      if (dist) residual4<true>(s_h, p, d, y, y1, vec, w);
-      else residual4<false>(s_h, p, d, y, y1, vec, w);
-      acc += (w[0] + w[1]) + (w[2] + w[3]);
-    }
+    for (int b = 0; b < n_batch; ++b) {
+      const int end = min(y0 + (b + 1) * batch, y1);
+      double one = 0.0;
+      for (int y = y0 + b * batch; y < end; y += step) {
+        double w[VF_GROUPS][4];
+        if (dist) weights<true>(s_h, p, d, y + 4 * lane, y1, vec, w);
+        else weights<false>(s_h, p, d, y + 4 * lane, y1, vec, w);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+        for (int g = 0; g < VF_GROUPS; ++g) one += (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
+      if (lane == 0) s_batch[warp][b] = one;
+      acc += one;
+    }
     sums = s_sum[parity];
     if (lane < C) cluster.map_shared_rank(sums, lane)[seg] = acc;
     cluster.sync();
@@ -290,7 +333,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
       double s = 0.0;
       if (lane < C)
 #pragma unroll
-        for (int k = 0; k < VF_WARPS; ++k) s += sums[lane * VF_WARPS + k];
+        for (int k = 0; k < WARPS; ++k) s += sums[lane * WARPS + k];
       double run = 0.0;
       for (int k = 0; k < C; ++k) {
         if (lane == 0) s_prefix[k] = run;
@@ -314,50 +357,51 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
     dist = s_drow[c] >= 0;
     drow = dist ? a.draft_probs + (size_t)s_drow[c] * a.ld_d : nullptr;
     double gone = 0.0;
+    bool unscaled = false;   // the last rejection's inv_z still stands for 1
     int took = -1;
     for (int x = n < t.path_w ? s_first[c] : VF_NODES; x < VF_NODES; x = s_sib[x]) {
       const int id = s_id[x];
       const double u = s_u[x];
       const bool again = rejected(s_h, id, 1);
-      bool changes = true;
       if (dist) {
         const double left = 1.0 - gone;
         const double scale = left > 0.0 ? 1.0 / left : 0.0;
         const double share = again ? 0.0 : s_d[x] * scale;
-        if (share > 0.0) {
-          const double r = residual<true>(s_h, id, s_p[x], s_d[x], again);
-          if (u * share < r) took = x;
-        } else {
-          changes = false;
-        }
-        if (took < 0 && changes) {
-          __syncthreads();          // every thread has read s_h
-          if (tid == 0) {
-            s_h.token[s_h.n] = id;
-            s_h.scale[s_h.n] = scale;
-            s_h.inv_z[s_h.n] = 1.0;
-            s_h.n += 1;
-          }
-          __syncthreads();
+        if (!(share > 0.0)) continue;
+        if (unscaled) {   // the last rejection's Z, now that a test needs it
           const double z = vocab_sum(prow, drow, true);
           if (tid == 0) s_h.inv_z[s_h.n - 1] = z > 0.0 ? 1.0 / z : 0.0;
           __syncthreads();
-          gone += s_d[x];
+          unscaled = false;
         }
+        if (u * share < residual(s_h, true, id, s_p[x], s_d[x])) {
+          took = x;
+          break;
+        }
+        __syncthreads();   // every thread has read s_h
+        if (tid == 0) {
+          s_h.token[s_h.n] = id;
+          s_h.scale[s_h.n] = scale;
+          s_h.inv_z[s_h.n] = 1.0;
+          s_h.n += 1;
+        }
+        __syncthreads();
+        unscaled = true;
+        gone += s_d[x];
       } else {
         const double r = again ? 0.0 : (double)s_p[x];
-        if (r > 0.0 && u * (1.0 - gone) < r) took = x;
-        else {
-          gone += r;
-          __syncthreads();
-          if (tid == 0) {
-            s_h.token[s_h.n] = id;
-            s_h.n += 1;
-          }
-          __syncthreads();
+        if (r > 0.0 && u * (1.0 - gone) < r) {
+          took = x;
+          break;
         }
+        gone += r;
+        __syncthreads();
+        if (tid == 0) {
+          s_h.token[s_h.n] = id;
+          s_h.n += 1;
+        }
+        __syncthreads();
       }
-      if (took >= 0) break;
     }
     if (took < 0) break;
     c = took;
@@ -368,13 +412,19 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
     __syncthreads();
   }
 
-  // ---- the sample: the CTA, then its warp, then the element in which the
-  // cumulative sum passes the target.  Each level searches its own running
-  // sums, so exactly one warp answers; a target that rounding leaves past a
-  // level's last sum takes the last positive one.
-  const double total = vocab_sum(prow, drow, dist);
+  // ---- the sample (r up to its scale): the CTA, its warp, the batch, then the
+  // element in which the cumulative sum passes the target.  Each level searches
+  // its own running sums, so exactly one warp answers; a target that rounding
+  // leaves past a level's last sum takes the last positive one.  A last rejection
+  // that leaves nothing (Z = 0) is taken back.
+  double total = vocab_sum(prow, drow, dist);
+  if (dist && s_h.n > 0 && !(total > 0.0)) {
+    if (tid == 0) s_h.inv_z[s_h.n - 1] = 0.0;
+    __syncthreads();
+    total = vocab_sum(prow, drow, dist);
+  }
   if (rank == 0) {
-    for (int k = n + tid; k < t.path_w; k += VF_THREADS) path[k] = -1;
+    for (int k = n + tid; k < t.path_w; k += THREADS) path[k] = -1;
     if (tid == 0) {
       t.n_accepted[seq] = n - 1;
       if (!(total > 0.0)) t.next_ids[seq] = -1;
@@ -384,52 +434,64 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
   const double aim = fmax((double)s_u[0] * total, 0.0);   // a NaN aims at 0
   const double lo = s_prefix[rank], hi = s_prefix[rank + 1];
   if (!(lo < hi && ((lo <= aim && aim < hi) || (aim >= total && hi >= total)))) return;
-  double at = aim - lo, run = 0.0;
-  int mine = 0;
-  double before = 0.0;
-  for (int w = 0; w < VF_WARPS; ++w) {
-    const double s = sums[rank * VF_WARPS + w];
-    if (!(s > 0.0)) continue;
-    mine = w;
-    before = run;
-    run += s;
-    if (at < run) break;
-  }
-  if (warp != mine) return;
-  at -= before;
-  run = 0.0;
+  double at = aim - lo;
+  // among n sums: the first whose running sum exceeds `at` (else the last positive
+  // one); `at` becomes relative to it
+  auto locate = [&](const double* v, int count) -> int {
+    double run = 0.0, before = 0.0;
+    int mine = 0;
+    for (int k = 0; k < count; ++k) {
+      const double s = v[k];
+      if (!(s > 0.0)) continue;
+      mine = k;
+      before = run;
+      run += s;
+      if (at < run) break;
+    }
+    at -= before;
+    return mine;
+  };
+  if (warp != locate(sums + rank * WARPS, WARPS)) return;
+  const int b = locate(s_batch[warp], n_batch);
   const bool vec = vec_p && (!dist || vec_d);
+  const int end = min(y0 + (b + 1) * batch, y1);
+  double run = 0.0;
   int next = -1;
-  for (int y = y0 + 4 * lane; y - 4 * lane < y1; y += 128) {
-    double w[4];
-    if (dist) residual4<true>(s_h, prow, drow, y, y1, vec, w);
-    else residual4<false>(s_h, prow, drow, y, y1, vec, w);
-    const double sum = (w[0] + w[1]) + (w[2] + w[3]);
-    double inc = sum;
+  for (int y = y0 + b * batch; y < end; y += step) {
+    double w[VF_GROUPS][4];
+    if (dist) weights<true>(s_h, prow, drow, y + 4 * lane, y1, vec, w);
+    else weights<false>(s_h, prow, drow, y + 4 * lane, y1, vec, w);
+    bool found = false;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    double cum = __shfl_up_sync(0xffffffffu, inc, 1);
-    cum = run + (lane > 0 ? cum : 0.0);
-    int hit = -1, pos = -1;
+    for (int g = 0; g < VF_GROUPS; ++g) {
+      if (found) break;
+      double inc = (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      cum += w[e];
-      if (w[e] > 0.0) {
-        pos = y + e;
-        if (hit < 0 && cum > at) hit = y + e;
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
       }
+      double cum = __shfl_up_sync(0xffffffffu, inc, 1);
+      cum = run + (lane > 0 ? cum : 0.0);
+      int hit = -1, pos = -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        cum += w[g][e];
+        if (w[g][e] > 0.0) {
+          pos = y + 128 * g + 4 * lane + e;
+          if (hit < 0 && cum > at) hit = pos;
+        }
+      }
+      const unsigned some = __ballot_sync(0xffffffffu, pos >= 0);
+      if (some) next = __shfl_sync(0xffffffffu, pos, 31 - __clz(some));
+      const unsigned any = __ballot_sync(0xffffffffu, hit >= 0);
+      if (any) {
+        next = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
+        found = true;
+      }
+      run += __shfl_sync(0xffffffffu, inc, 31);
     }
-    const unsigned some = __ballot_sync(0xffffffffu, pos >= 0);
-    if (some) next = __shfl_sync(0xffffffffu, pos, 31 - __clz(some));
-    const unsigned any = __ballot_sync(0xffffffffu, hit >= 0);
-    if (any) {
-      next = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
-      break;
-    }
-    run += __shfl_sync(0xffffffffu, inc, 31);
+    if (found) break;
   }
   if (lane == 0) t.next_ids[seq] = next;
 }
@@ -456,15 +518,22 @@ int verify_greedy_launch(const TreeArgs& t, const int* target_ids, int max_q, cu
 int verify_launch(const VerifyArgs& a, int max_q, cudaStream_t st) {
   if (int rc = check_tree(a.t, max_q)) return rc;
   if (a.t.n_seqs == 0) return TB_OK;
-  if (a.vocab <= 0 || a.ld_p < a.vocab || a.probs == nullptr || a.uniforms == nullptr)
+  if (a.vocab <= 0 || a.vocab > (1 << 28) || a.ld_p < a.vocab || a.probs == nullptr || a.uniforms == nullptr)
     return arg_err("probs / vocab / uniforms");
   if ((a.draft_probs == nullptr) != (a.draft_rows == nullptr))
     return arg_err("draft_probs and draft_rows go together");
   if (a.draft_probs != nullptr && (a.ld_d < a.vocab || a.n_draft_rows < 0))
     return arg_err("draft_probs shape");
-  const int cluster = VF_MAX_CLUSTER;
-  if (a.t.n_seqs > 0x7fffffff / cluster) return arg_err("n_seqs");
-  return launch_pdl(verify_kernel, dim3(a.t.n_seqs * cluster), dim3(VF_THREADS), 0, st, cluster,
+  // few sequences: wide CTAs, two loads in flight cover a segment; many: one
+  // wave of smaller ones
+  const int n = a.t.n_seqs;
+  if (n > 0x7fffffff / VF_MAX_CLUSTER) return arg_err("n_seqs");
+  int cluster = 8;
+  if (n * 8 <= 148)
+    return launch_pdl(verify_kernel<512, 1>, dim3(n * cluster), dim3(512), 0, st, cluster,
+                      "draft verification launch", a);
+  while (cluster > 1 && n * (long long)cluster > 148 * 3) cluster /= 2;
+  return launch_pdl(verify_kernel<256, 3>, dim3(n * cluster), dim3(256), 0, st, cluster,
                     "draft verification launch", a);
 }
 

@@ -8,6 +8,7 @@ allocates per call except when no arena is given).
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
@@ -167,34 +168,44 @@ def _device(t: torch.Tensor) -> int:
     return dev
 
 
-def _in(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev: int) -> int:
-    """Data pointer of an argument of the given type, shape (None: any size)
-    and device whose last dimension is contiguous."""
-    got = t.shape
-    if t.dtype is not dtype or t.get_device() != dev or len(got) != len(shape):
-        raise ValueError(f"{name}: expected a {len(shape)}-d {dtype} tensor on cuda:{dev}, got "
-                         f"{tuple(got)} {t.dtype} on {t.device}")
-    for g, w in zip(got, shape):
-        if w is not None and g != w:
-            raise ValueError(f"{name}: expected shape {shape}, got {tuple(got)}")
-    if got and got[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
-    return t.data_ptr()
+# One function per kind of argument, a single condition each: a decode step's
+# calls are a few microseconds of GPU work, so the host's share counts.
+
+def _refuse(name: str, t: torch.Tensor, want: str, dev: int):
+    raise ValueError(f"{name}: expected {want} on cuda:{dev}, got {tuple(t.shape)} {t.dtype} on "
+                     f"{t.device}, strides {t.stride()}")
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Row pitch of a 2-d argument in elements (its width where it has one row)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _vec(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev: int) -> int:
+    """Data pointer of a contiguous argument of exactly this shape."""
+    if (t.dtype is dtype and t.shape == shape and t.get_device() == dev
+            and t.is_contiguous()):
+        return t.data_ptr()
+    _refuse(name, t, f"a contiguous {shape} {dtype} tensor", dev)
+
+
+def _mat(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int | None, dev: int):
+    """(pointer, row pitch, columns) of a 2-d argument with contiguous rows."""
+    shape = t.shape
+    if t.dtype is dtype and len(shape) == 2 and t.get_device() == dev:
+        n, cols = shape
+        pitch, step = t.stride()
+        if (rows is None or n == rows) and (step == 1 or cols <= 1):
+            return t.data_ptr(), (pitch if n > 1 else cols), cols
+    _refuse(name, t, f"a 2-d {dtype} tensor of {'any' if rows is None else rows} contiguous rows",
+            dev)
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream     # torch.cuda.current_stream without its object
 
 
 def _run_on(dev: int, what: str, fn, *args) -> None:
     """Call ``fn(*args, stream)`` on device ``dev``'s current stream."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
     if dev == torch.cuda.current_device():
-        rc = fn(*args, stream)
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, stream)
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         N.check(rc, what)
 
@@ -214,39 +225,35 @@ def paged_attention_tree(q, out, kv_pool, *, n_q_heads, n_kv_heads, head_dim, bl
     caller knows them (they only choose how a context is shared out)."""
     lib = N.load()
     dev = _device(q)
-    rows = q.shape[0]
-    n = ctx_len.shape[0]
-    words = tree_mask.shape[-1]
-    bf = torch.bfloat16
-    width = n_q_heads * head_dim
-    qp = _in("q", q, bf, (rows, width), dev)
-    op = _in("out", out, bf, (rows, width), dev)
-    pp = _in("kv_pool", kv_pool, bf, (None, 2, n_kv_heads, block_size, head_dim), dev)
-    if not kv_pool.is_contiguous():
-        raise ValueError("kv_pool must be contiguous")
-    i32 = torch.int32
-    bp = _in("block_tables", block_tables, i32, (n, None), dev)
-    sp = _in("q_start", q_start, i32, (n,), dev)
-    lp = _in("q_len", q_len, i32, (n,), dev)
-    cp = _in("ctx_len", ctx_len, i32, (n,), dev)
-    mp = _in("tree_mask", tree_mask, torch.int64, (rows, words), dev)
-    if max_q is None:
-        max_q = min(rows, 64 * words)
-    _run_on(dev, "tb_paged_attention_tree", lib.tb_paged_attention_tree, qp, _ld(q), op, _ld(out),
-            rows, pp, kv_pool.shape[0], n_q_heads, n_kv_heads, head_dim, block_size, bp,
-            _ld(block_tables), block_tables.shape[1], sp, lp, cp, n, mp, _ld(tree_mask), words,
-            max_q, max_ctx, ctx_total)
+    rows, n = len(q), len(ctx_len)
+    i32, bf = torch.int32, torch.bfloat16
+    qp, ldq, cols = _mat("q", q, bf, rows, dev)
+    op, ldo, ocols = _mat("out", out, bf, rows, dev)
+    if cols != n_q_heads * head_dim or ocols != cols:
+        raise ValueError(f"q and out: expected {n_q_heads * head_dim} columns, got {cols} and {ocols}")
+    blocks = len(kv_pool)
+    pp = _vec("kv_pool", kv_pool, bf, (blocks, 2, n_kv_heads, block_size, head_dim), dev)
+    bp, ldb, width = _mat("block_tables", block_tables, i32, n, dev)
+    mp, ldm, words = _mat("tree_mask", tree_mask, torch.int64, rows, dev)
+    seqs = (n,)
+    _run_on(dev, "tb_paged_attention_tree", lib.tb_paged_attention_tree, qp, ldq, op, ldo, rows, pp,
+            blocks, n_q_heads, n_kv_heads, head_dim, block_size, bp, ldb, width,
+            _vec("q_start", q_start, i32, seqs, dev), _vec("q_len", q_len, i32, seqs, dev),
+            _vec("ctx_len", ctx_len, i32, seqs, dev), n, mp, ldm, words,
+            min(rows, 64 * words) if max_q is None else max_q, max_ctx, ctx_total)
 
 
 def _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev):
-    """Pointers and sizes of the arguments both verifications share."""
+    """Sizes and pointers of the arguments both verifications share."""
     i32 = torch.int32
-    rows, n = ids.shape[0], q_len.shape[0]
-    return (rows, n,
-            (_in("ids", ids, i32, (rows,), dev), _in("parents", parents, i32, (rows,), dev),
-             _in("q_start", q_start, i32, (n,), dev), _in("q_len", q_len, i32, (n,), dev)),
-            (_in("n_accepted", n_accepted, i32, (n,), dev), _in("path", path, i32, (n, None), dev),
-             _ld(path), path.shape[1], _in("next_ids", next_ids, i32, (n,), dev)))
+    rows, seqs = ids.shape, q_len.shape
+    if len(rows) != 1 or len(seqs) != 1:
+        raise ValueError("ids and q_len: expected 1-d tensors")
+    return (rows, seqs[0],
+            (_vec("ids", ids, i32, rows, dev), _vec("parents", parents, i32, rows, dev),
+             _vec("q_start", q_start, i32, seqs, dev), _vec("q_len", q_len, i32, seqs, dev)),
+            (_vec("n_accepted", n_accepted, i32, seqs, dev),
+             *_mat("path", path, i32, seqs[0], dev), _vec("next_ids", next_ids, i32, seqs, dev)))
 
 
 def verify_drafts_greedy(ids, parents, q_start, q_len, target_ids, n_accepted, path, next_ids, *,
@@ -259,9 +266,9 @@ def verify_drafts_greedy(ids, parents, q_start, q_len, target_ids, n_accepted, p
     lib = N.load()
     dev = _device(ids)
     rows, n, tree, outs = _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev)
-    tp = _in("target_ids", target_ids, torch.int32, (rows,), dev)
-    _run_on(dev, "tb_verify_drafts_greedy", lib.tb_verify_drafts_greedy, *tree, n, rows, max_q, tp,
-            *outs)
+    tp = _vec("target_ids", target_ids, torch.int32, rows, dev)
+    _run_on(dev, "tb_verify_drafts_greedy", lib.tb_verify_drafts_greedy, *tree, n, rows[0], max_q,
+            tp, *outs)
 
 
 def verify_drafts(ids, parents, q_start, q_len, probs, uniforms, n_accepted, path, next_ids, *,
@@ -279,17 +286,18 @@ def verify_drafts(ids, parents, q_start, q_len, probs, uniforms, n_accepted, pat
     dev = _device(ids)
     rows, n, tree, outs = _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev)
     f32 = torch.float32
-    pp = _in("probs", probs, f32, (rows, None), dev)
-    up = _in("uniforms", uniforms, f32, (rows,), dev)
-    vocab = probs.shape[1]
+    pp, ldp, vocab = _mat("probs", probs, f32, rows[0], dev)
+    up = _vec("uniforms", uniforms, f32, rows, dev)
     if (draft_probs is None) != (draft_rows is None):
         raise ValueError("draft_probs and draft_rows go together")
     draft = (None, 0, 0, None)
     if draft_probs is not None:
-        draft = (_in("draft_probs", draft_probs, f32, (None, vocab), dev), _ld(draft_probs),
-                 draft_probs.shape[0], _in("draft_rows", draft_rows, torch.int32, (rows,), dev))
-    _run_on(dev, "tb_verify_drafts", lib.tb_verify_drafts, *tree, n, rows, max_q, pp, _ld(probs),
-            vocab, *draft, up, *outs)
+        dp, ldd, cols = _mat("draft_probs", draft_probs, f32, None, dev)
+        if cols != vocab:
+            raise ValueError(f"draft_probs: expected {vocab} columns, got {cols}")
+        draft = (dp, ldd, len(draft_probs), _vec("draft_rows", draft_rows, torch.int32, rows, dev))
+    _run_on(dev, "tb_verify_drafts", lib.tb_verify_drafts, *tree, n, rows[0], max_q, pp, ldp, vocab,
+            *draft, up, *outs)
 
 
 class KVPools:
@@ -299,39 +307,43 @@ class KVPools:
     def __init__(self, pools):
         """``pools``: a list of ``[num_blocks, 2, n_kv, block_size, head_dim]``
         bf16 tensors, or one tensor with the layers stacked in front."""
-        stacked = isinstance(pools, torch.Tensor)
-        if stacked and pools.dim() != 6:
-            raise ValueError("stacked pools: expected [layers, num_blocks, 2, n_kv, block_size, head_dim]")
-        if not stacked:
-            pools = list(pools)
-        self.pools = pools
-        self.n_layers = len(pools)
-        if self.n_layers == 0:
-            raise ValueError("no pools")
-        first = pools[0]
-        self.device = _device(first)
-        shape = first.shape
-        if len(shape) != 5 or shape[1] != 2:
-            raise ValueError(f"pools: expected [num_blocks, 2, n_kv, block_size, head_dim], got {tuple(shape)}")
-        if stacked:
-            if first.dtype is not torch.bfloat16 or not first.is_contiguous():
-                raise ValueError("pools must be bf16 and contiguous")
-            step = pools.stride(0) * 2
-            if self.n_layers > 1 and step < first.numel() * 2:
+        if isinstance(pools, torch.Tensor):
+            shape, pitch = pools.shape, pools.stride()
+            if len(shape) != 6 or shape[2] != 2:
+                raise ValueError("stacked pools: expected [layers, num_blocks, 2, n_kv, block_size, "
+                                 f"head_dim], got {tuple(shape)}")
+            layers, blocks, _, heads, size, dim = shape
+            token = size * dim
+            if pools.dtype is not torch.bfloat16 or (
+                    pitch[1:] != (2 * heads * token, heads * token, token, dim, 1)
+                    and not (layers and pools[0].is_contiguous())):
+                raise ValueError("pools must be bf16, each layer's contiguous")
+            step = pitch[0] * 2
+            if layers > 1 and step < blocks * heads * token * 4:
                 raise ValueError("pools: layers overlap")
-            p0 = first.data_ptr()
-            ptrs = [p0 + i * step for i in range(self.n_layers)]
+            first = pools.data_ptr()
+            ptrs = range(first, first + layers * step, step) if layers > 1 else (first,) * layers
+            self.device = _device(pools)
         else:
+            pools = list(pools)
+            shape = pools[0].shape if pools else ()
+            if len(shape) != 5 or shape[1] != 2:
+                raise ValueError("pools: expected tensors [num_blocks, 2, n_kv, block_size, head_dim], "
+                                 f"got {tuple(shape)}")
+            layers = len(pools)
+            blocks, _, heads, size, dim = shape
+            self.device = _device(pools[0])
             for t in pools:
                 if (t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous()
                         or t.get_device() != self.device):
                     raise ValueError("pools must be contiguous bf16 tensors of one shape and device")
             ptrs = [t.data_ptr() for t in pools]
-            if len(set(ptrs)) != len(ptrs):
+            if len(set(ptrs)) != layers:
                 raise ValueError("pools: a layer is listed twice")
-        self.num_blocks, _, self.n_kv_heads, self.block_size, self.head_dim = shape
-        self.array = (ctypes.c_void_p * self.n_layers)(*ptrs)
-        self.args = (self.array, self.n_layers, *(int(shape[i]) for i in (0, 2, 3, 4)))
+        self.pools = pools
+        self._addresses = array("Q", ptrs)      # what the first of args points to
+        # the C calls' first arguments: the addresses, the layers, a pool's shape
+        self.args = (self._addresses.buffer_info()[0], layers, blocks, heads, size, dim)
 
 
 def _pools(pools) -> KVPools:
@@ -347,14 +359,14 @@ def keep_kv_path(pools, *, block_tables, q_len, ctx_len, path, n_accepted):
     kv = _pools(pools)
     dev = kv.device
     i32 = torch.int32
-    n = q_len.shape[0]
-    bp = _in("block_tables", block_tables, i32, (n, None), dev)
-    lp = _in("q_len", q_len, i32, (n,), dev)
-    cp = _in("ctx_len", ctx_len, i32, (n,), dev)
-    pp = _in("path", path, i32, (n, None), dev)
-    ap = _in("n_accepted", n_accepted, i32, (n,), dev)
-    _run_on(dev, "tb_keep_kv_path", lib.tb_keep_kv_path, *kv.args, bp, _ld(block_tables),
-            block_tables.shape[1], lp, cp, pp, _ld(path), path.shape[1], ap, n)
+    seqs = q_len.shape
+    if len(seqs) != 1:
+        raise ValueError("q_len: expected a 1-d tensor")
+    _run_on(dev, "tb_keep_kv_path", lib.tb_keep_kv_path, *kv.args,
+            *_mat("block_tables", block_tables, i32, seqs[0], dev),
+            _vec("q_len", q_len, i32, seqs, dev), _vec("ctx_len", ctx_len, i32, seqs, dev),
+            *_mat("path", path, i32, seqs[0], dev),
+            _vec("n_accepted", n_accepted, i32, seqs, dev), seqs[0])
 
 
 def copy_kv_blocks(pools, pairs):
@@ -364,10 +376,9 @@ def copy_kv_blocks(pools, pairs):
     status word.  ``pools``: ``KVPools``, or what it takes."""
     lib = N.load()
     kv = _pools(pools)
-    pp = _in("pairs", pairs, torch.int32, (None, 2), kv.device)
-    if not pairs.is_contiguous():
-        raise ValueError("pairs must be contiguous")
-    _run_on(kv.device, "tb_copy_kv_blocks", lib.tb_copy_kv_blocks, *kv.args, pp, pairs.shape[0])
+    n = len(pairs)
+    _run_on(kv.device, "tb_copy_kv_blocks", lib.tb_copy_kv_blocks, *kv.args,
+            _vec("pairs", pairs, torch.int32, (n, 2), kv.device), n)
 
 
 def embed(ids, emb, g, h, hg, sq):
