@@ -80,6 +80,22 @@ int smem_attr_once(void (*kern)(KArgs...), int bytes, std::atomic<unsigned long 
   return 0;
 }
 
+// Allow clusters of more than 8 CTAs (up to 16) for `kern`, once per device
+// (`devs` as in smem_attr_once).
+template <typename... KArgs>
+int wide_cluster_once(void (*kern)(KArgs...), std::atomic<unsigned long long>& devs,
+                      const char* what) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return host_err(e, what);
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (bit && (devs.load(std::memory_order_acquire) & bit)) return 0;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return host_err(e, what);
+  devs.fetch_or(bit, std::memory_order_release);
+  return 0;
+}
+
 struct GemmArgs;
 int gemm_launch(int epi, int bn, const void* A, int lda, const void* B, int ldb, GemmArgs g,
                 cudaStream_t stream);

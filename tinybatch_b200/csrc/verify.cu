@@ -35,7 +35,6 @@ namespace tb {
 constexpr int VF_NODES = 256;      // nodes of a sequence's tree
 constexpr int VF_MAX_WARPS = 16;
 constexpr int VF_MAX_CLUSTER = 16;
-constexpr int VF_GROUPS = 4;       // 128-token groups whose loads a warp has in flight
 constexpr int VF_BATCHES = 32;     // sums a warp keeps of its part of the vocabulary
 
 struct TreeArgs {
@@ -155,28 +154,28 @@ __device__ __forceinline__ float4 load4(const float* row, int y, int end, bool v
                      y + 2 < end ? __ldg(row + y + 2) : 0.f, y + 3 < end ? __ldg(row + y + 3) : 0.f);
 }
 
-// r of tokens y + 128 g .. + 3, g < VF_GROUPS (y already the lane's; 0 from
+// r of tokens y + 128 g .. + 3, g < GROUPS (y already the lane's; 0 from
 // `end` on).  All loads are issued before the first is used.
-template <bool DIST>
+template <bool DIST, int GROUPS>
 __device__ __forceinline__ void weights(const Rejections& h, const float* p, const float* d, int y,
                                         int end, bool vec, double (*w)[4]) {
-  float4 pv[VF_GROUPS], dv[VF_GROUPS];
+  float4 pv[GROUPS], dv[GROUPS];
 #pragma unroll
-  for (int g = 0; g < VF_GROUPS; ++g) pv[g] = load4(p, y + 128 * g, end, vec);
+  for (int g = 0; g < GROUPS; ++g) pv[g] = load4(p, y + 128 * g, end, vec);
   if (DIST)
 #pragma unroll
-    for (int g = 0; g < VF_GROUPS; ++g) dv[g] = load4(d, y + 128 * g, end, vec);
+    for (int g = 0; g < GROUPS; ++g) dv[g] = load4(d, y + 128 * g, end, vec);
 #pragma unroll
-  for (int g = 0; g < VF_GROUPS; ++g)
+  for (int g = 0; g < GROUPS; ++g)
     w[g][0] = pv[g].x, w[g][1] = pv[g].y, w[g][2] = pv[g].z, w[g][3] = pv[g].w;
   // the warp's stretch holds a rejected token (rare): only then are tokens compared
-  const bool special = rejected(h, y & ~127, 128 * VF_GROUPS);
+  const bool special = rejected(h, y & ~127, 128 * GROUPS);
   for (int k = 0; k < h.n; ++k) {
     if (DIST) {
       const double sc = h.scale[k], iz = h.inv_z[k];
       if (iz > 0.0) {
 #pragma unroll
-        for (int g = 0; g < VF_GROUPS; ++g) {
+        for (int g = 0; g < GROUPS; ++g) {
           w[g][0] = fmax(w[g][0] - dv[g].x * sc, 0.0);
           w[g][1] = fmax(w[g][1] - dv[g].y * sc, 0.0);
           w[g][2] = fmax(w[g][2] - dv[g].z * sc, 0.0);
@@ -184,7 +183,7 @@ __device__ __forceinline__ void weights(const Rejections& h, const float* p, con
         }
         if (iz != 1.0)
 #pragma unroll
-          for (int g = 0; g < VF_GROUPS; ++g)
+          for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[g][e] *= iz;
       }
@@ -192,7 +191,7 @@ __device__ __forceinline__ void weights(const Rejections& h, const float* p, con
     if (special) {
       const int x = h.token[k] - y;
 #pragma unroll
-      for (int g = 0; g < VF_GROUPS; ++g) {
+      for (int g = 0; g < GROUPS; ++g) {
         if (DIST) {
           if (x == 128 * g) dv[g].x = 0.f;
           if (x == 128 * g + 1) dv[g].y = 0.f;
@@ -213,18 +212,18 @@ __device__ __forceinline__ void weights(const Rejections& h, const float* p, con
 // loads, same arithmetic), so the cluster only meets for sums over the
 // vocabulary: one for each rejection whose Z a later sibling's test needs, one
 // for the sample.
-template <int THREADS, int MIN_CTAS>
+// GROUPS: 128-token groups whose loads a warp has in flight.
+template <int THREADS, int MIN_CTAS, int GROUPS>
 __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyArgs a) {
   namespace cg = cooperative_groups;
   constexpr int WARPS = THREADS / 32;
   static_assert(WARPS <= VF_MAX_WARPS, "sum slots");
-  __shared__ int s_id[VF_NODES], s_first[VF_NODES], s_sib[VF_NODES], s_par[VF_NODES];
+  __shared__ int s_id[VF_NODES], s_par[VF_NODES], s_drow[VF_NODES];
   __shared__ float s_p[VF_NODES], s_d[VF_NODES], s_u[VF_NODES];
-  __shared__ int s_drow[VF_NODES];
   __shared__ Rejections s_h;
+  __shared__ int s_node, s_sum_wanted;
   __shared__ double s_sum[2][VF_MAX_CLUSTER * WARPS];
   __shared__ double s_batch[WARPS][VF_BATCHES];
-  __shared__ double s_prefix[VF_MAX_CLUSTER + 1];
   cg::cluster_group cluster = cg::this_cluster();
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
@@ -267,31 +266,20 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
     s_id[i] = id;
     s_u[i] = a.uniforms[q0 + i];
     s_drow[i] = dr;
-    s_first[i] = VF_NODES;
-    s_p[i] = p >= 0 ? a.probs[(size_t)(q0 + p) * a.ld_p + id] : 0.f;
   }
+  if (tid == 0) s_h.n = 0;
   __syncthreads();
   for (int i = tid; i < ql; i += THREADS) {
     const int p = s_par[i];
-    int sib = VF_NODES;
-    if (p >= 0) {
-      atomicMin(&s_first[p], i);
-      const int dr = s_drow[p];
-      s_d[i] = dr >= 0 ? a.draft_probs[(size_t)dr * a.ld_d + s_id[i]] : 0.f;
-      for (int j = i + 1; j < ql; ++j)
-        if (s_par[j] == p) {
-          sib = j;
-          break;
-        }
-    }
-    s_sib[i] = sib;
+    const int dr = p >= 0 ? s_drow[p] : -1;
+    s_p[i] = p >= 0 ? a.probs[(size_t)(q0 + p) * a.ld_p + s_id[i]] : 0.f;
+    s_d[i] = dr >= 0 ? a.draft_probs[(size_t)dr * a.ld_d + s_id[i]] : 0.f;
   }
-  if (tid == 0) s_h.n = 0;
   __syncthreads();
   cluster.barrier_wait(std::move(started));
 
   // this warp's segment of the vocabulary, in batches
-  const int step = 128 * VF_GROUPS;
+  const int step = 128 * GROUPS;
   const int n_seg = C * WARPS;
   const int batch = ((a.vocab + n_seg * VF_BATCHES - 1) / (n_seg * VF_BATCHES) + step - 1) / step * step;
   const int n_batch = ((a.vocab + n_seg - 1) / n_seg + batch - 1) / batch;
@@ -305,9 +293,8 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
   double* sums = s_sum[0];
 
   // Sum over the vocabulary of r with the rejections of s_h applied.  All
-  // threads of the cluster call it; every one gets the same sum.  s_batch: the
-  // batches' sums; s_prefix: the CTAs' exclusive prefix sums, summed in rank
-  // order (so they never decrease), and the total.
+  // threads of the cluster call it; every one gets the same sum.  sums: the
+  // segments' sums; s_batch: those of this CTA's batches.
   auto vocab_sum = [&](const float* p, const float* d, bool dist) -> double {
     double acc = 0.0;
     const bool vec = vec_p && (!dist || vec_d);
@@ -315,11 +302,11 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
       const int end = min(y0 + (b + 1) * batch, y1);
       double one = 0.0;
       for (int y = y0 + b * batch; y < end; y += step) {
-        double w[VF_GROUPS][4];
-        if (dist) weights<true>(s_h, p, d, y + 4 * lane, y1, vec, w);
-        else weights<false>(s_h, p, d, y + 4 * lane, y1, vec, w);
+        double w[GROUPS][4];
+        if (dist) weights<true, GROUPS>(s_h, p, d, y + 4 * lane, y1, vec, w);
+        else weights<false, GROUPS>(s_h, p, d, y + 4 * lane, y1, vec, w);
 #pragma unroll
-        for (int g = 0; g < VF_GROUPS; ++g) one += (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
+        for (int g = 0; g < GROUPS; ++g) one += (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
@@ -329,149 +316,170 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
     sums = s_sum[parity];
     if (lane < C) cluster.map_shared_rank(sums, lane)[seg] = acc;
     cluster.sync();
-    if (warp == 0) {
-      double s = 0.0;
-      if (lane < C)
+    parity ^= 1;   // the other buffer next: a CTA may still be reading this one
+    double all = 0.0;
+    for (int k = lane; k < n_seg; k += 32) all += sums[k];
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) s += sums[lane * WARPS + k];
-      double run = 0.0;
-      for (int k = 0; k < C; ++k) {
-        if (lane == 0) s_prefix[k] = run;
-        run += __shfl_sync(0xffffffffu, s, k);
-      }
-      if (lane == 0) s_prefix[C] = run;
-    }
-    __syncthreads();
-    parity ^= 1;   // the other buffer: a CTA may still be reading this one
-    return s_prefix[C];
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    return all;
   };
 
-  // ---- the walk
-  int c = 0, n = 1;
-  bool dist = false;
-  const float* prow = a.probs;
-  const float* drow = nullptr;
+  // ---- the walk, by the first warp of every CTA; the others join for a sum
+  int c = 0, n = 1, x = 0;         // node, path length, last child looked at
+  double gone = 0.0;
+  bool unscaled = false;           // the last rejection's inv_z still stands for 1
   if (rank == 0 && tid == 0) path[0] = 0;
   while (true) {
-    prow = a.probs + (size_t)(q0 + c) * a.ld_p;
-    dist = s_drow[c] >= 0;
-    drow = dist ? a.draft_probs + (size_t)s_drow[c] * a.ld_d : nullptr;
-    double gone = 0.0;
-    bool unscaled = false;   // the last rejection's inv_z still stands for 1
-    int took = -1;
-    for (int x = n < t.path_w ? s_first[c] : VF_NODES; x < VF_NODES; x = s_sib[x]) {
-      const int id = s_id[x];
-      const double u = s_u[x];
-      const bool again = rejected(s_h, id, 1);
-      if (dist) {
-        const double left = 1.0 - gone;
-        const double scale = left > 0.0 ? 1.0 / left : 0.0;
-        const double share = again ? 0.0 : s_d[x] * scale;
-        if (!(share > 0.0)) continue;
-        if (unscaled) {   // the last rejection's Z, now that a test needs it
-          const double z = vocab_sum(prow, drow, true);
-          if (tid == 0) s_h.inv_z[s_h.n - 1] = z > 0.0 ? 1.0 / z : 0.0;
-          __syncthreads();
+    if (warp == 0) {
+      bool sum = false;
+      while (true) {
+        // the next child in node order
+        int child = -1;
+        for (int i0 = (x + 1) & ~31; i0 < ql && n < t.path_w && child < 0; i0 += 32) {
+          const int i = i0 + lane;
+          const unsigned hit = __ballot_sync(0xffffffffu, i < ql && i > x && s_par[i] == c);
+          if (hit) child = i0 + __ffs(hit) - 1;
+        }
+        if (child < 0) break;
+        const int id = s_id[child];
+        const double u = s_u[child];
+        const bool again = rejected(s_h, id, 1);
+        bool took;
+        if (s_drow[c] >= 0) {
+          const double left = 1.0 - gone;
+          const double scale = left > 0.0 ? 1.0 / left : 0.0;
+          const double share = again ? 0.0 : s_d[child] * scale;
+          x = child;
+          if (!(share > 0.0)) continue;
+          if (unscaled) {          // the last rejection's Z, now that a test needs it
+            x = child - 1;
+            sum = true;
+            break;
+          }
+          took = u * share < residual(s_h, true, id, s_p[child], s_d[child]);
+          if (!took) {
+            __syncwarp();
+            if (lane == 0) {
+              s_h.token[s_h.n] = id;
+              s_h.scale[s_h.n] = scale;
+              s_h.inv_z[s_h.n] = 1.0;
+              s_h.n += 1;
+            }
+            __syncwarp();
+            unscaled = true;
+            gone += s_d[child];
+          }
+        } else {
+          const double r = again ? 0.0 : (double)s_p[child];
+          x = child;
+          took = r > 0.0 && u * (1.0 - gone) < r;
+          if (!took) {
+            gone += r;
+            __syncwarp();
+            if (lane == 0) {
+              s_h.token[s_h.n] = id;
+              s_h.n += 1;
+            }
+            __syncwarp();
+          }
+        }
+        if (took) {
+          c = child;
+          gone = 0.0;
           unscaled = false;
+          if (rank == 0 && lane == 0) path[n] = c;
+          ++n;
+          __syncwarp();
+          if (lane == 0) s_h.n = 0;
+          __syncwarp();
         }
-        if (u * share < residual(s_h, true, id, s_p[x], s_d[x])) {
-          took = x;
-          break;
-        }
-        __syncthreads();   // every thread has read s_h
-        if (tid == 0) {
-          s_h.token[s_h.n] = id;
-          s_h.scale[s_h.n] = scale;
-          s_h.inv_z[s_h.n] = 1.0;
-          s_h.n += 1;
-        }
-        __syncthreads();
-        unscaled = true;
-        gone += s_d[x];
-      } else {
-        const double r = again ? 0.0 : (double)s_p[x];
-        if (r > 0.0 && u * (1.0 - gone) < r) {
-          took = x;
-          break;
-        }
-        gone += r;
-        __syncthreads();
-        if (tid == 0) {
-          s_h.token[s_h.n] = id;
-          s_h.n += 1;
-        }
-        __syncthreads();
+      }
+      if (lane == 0) {
+        s_node = c;
+        s_sum_wanted = sum;
       }
     }
-    if (took < 0) break;
-    c = took;
-    if (rank == 0 && tid == 0) path[n] = c;
-    ++n;
     __syncthreads();
-    if (tid == 0) s_h.n = 0;
-    __syncthreads();
+    c = s_node;
+    if (!s_sum_wanted) break;
+    const double z = vocab_sum(a.probs + (size_t)(q0 + c) * a.ld_p,
+                               a.draft_probs + (size_t)s_drow[c] * a.ld_d, true);
+    // (past the cluster's barrier no warp of this CTA reads s_h or the command)
+    if (warp == 0) {
+      if (lane == 0) s_h.inv_z[s_h.n - 1] = z > 0.0 ? 1.0 / z : 0.0;
+      __syncwarp();
+      unscaled = false;
+    }
   }
 
-  // ---- the sample (r up to its scale): the CTA, its warp, the batch, then the
-  // element in which the cumulative sum passes the target.  Each level searches
-  // its own running sums, so exactly one warp answers; a target that rounding
-  // leaves past a level's last sum takes the last positive one.  A last rejection
-  // that leaves nothing (Z = 0) is taken back.
+  // ---- the sample (r up to its scale).  A last rejection that leaves nothing
+  // (Z = 0) is taken back.
+  const float* prow = a.probs + (size_t)(q0 + c) * a.ld_p;
+  const bool dist = s_drow[c] >= 0;
+  const float* drow = dist ? a.draft_probs + (size_t)s_drow[c] * a.ld_d : nullptr;
   double total = vocab_sum(prow, drow, dist);
   if (dist && s_h.n > 0 && !(total > 0.0)) {
+    __syncthreads();
     if (tid == 0) s_h.inv_z[s_h.n - 1] = 0.0;
     __syncthreads();
     total = vocab_sum(prow, drow, dist);
   }
-  if (rank == 0) {
-    for (int k = n + tid; k < t.path_w; k += THREADS) path[k] = -1;
-    if (tid == 0) {
+  if (rank == 0 && warp == 0) {
+    for (int k = n + lane; k < t.path_w; k += 32) path[k] = -1;
+    if (lane == 0) {
       t.n_accepted[seq] = n - 1;
       if (!(total > 0.0)) t.next_ids[seq] = -1;
     }
   }
   if (!(total > 0.0)) return;
-  const double aim = fmax((double)s_u[0] * total, 0.0);   // a NaN aims at 0
-  const double lo = s_prefix[rank], hi = s_prefix[rank + 1];
-  if (!(lo < hi && ((lo <= aim && aim < hi) || (aim >= total && hi >= total)))) return;
-  double at = aim - lo;
-  // among n sums: the first whose running sum exceeds `at` (else the last positive
-  // one); `at` becomes relative to it
-  auto locate = [&](const double* v, int count) -> int {
-    double run = 0.0, before = 0.0;
-    int mine = 0;
-    for (int k = 0; k < count; ++k) {
-      const double s = v[k];
-      if (!(s > 0.0)) continue;
-      mine = k;
-      before = run;
-      run += s;
-      if (at < run) break;
+  // The CTA, its warp, its batch, then the element in which the cumulative sum
+  // passes the target.  Among the sums of a level (one a lane) that is the last
+  // positive one whose exclusive prefix does not exceed what is left of the
+  // target: some lane always qualifies, and every warp of the cluster picks the
+  // same one, however the prefixes are rounded.
+  double at = fmax((double)s_u[0] * total, 0.0);   // a NaN aims at 0
+  auto locate = [&](double v) -> int {
+    double inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
     }
-    at -= before;
-    return mine;
+    double ex = __shfl_up_sync(0xffffffffu, inc, 1);
+    if (lane == 0) ex = 0.0;
+    const int k = 31 - __clz(__ballot_sync(0xffffffffu, v > 0.0 && ex <= at));
+    at = k < 0 ? at : at - __shfl_sync(0xffffffffu, ex, k & 31);
+    return k;
   };
-  if (warp != locate(sums + rank * WARPS, WARPS)) return;
-  const int b = locate(s_batch[warp], n_batch);
+  double v = 0.0;
+  if (lane < C)
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) v += sums[lane * WARPS + k];
+  if (locate(v) != rank) return;
+  if (locate(lane < WARPS ? sums[rank * WARPS + lane] : 0.0) != warp) return;
+  const int b = locate(lane < n_batch ? s_batch[warp][lane] : 0.0);
+  if (b < 0) return;
   const bool vec = vec_p && (!dist || vec_d);
   const int end = min(y0 + (b + 1) * batch, y1);
   double run = 0.0;
   int next = -1;
   for (int y = y0 + b * batch; y < end; y += step) {
-    double w[VF_GROUPS][4];
-    if (dist) weights<true>(s_h, prow, drow, y + 4 * lane, y1, vec, w);
-    else weights<false>(s_h, prow, drow, y + 4 * lane, y1, vec, w);
+    double w[GROUPS][4], inc[GROUPS];
+    if (dist) weights<true, GROUPS>(s_h, prow, drow, y + 4 * lane, y1, vec, w);
+    else weights<false, GROUPS>(s_h, prow, drow, y + 4 * lane, y1, vec, w);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) inc[g] = (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const double up = __shfl_up_sync(0xffffffffu, inc[g], o);
+        if (lane >= o) inc[g] += up;
+      }
     bool found = false;
 #pragma unroll
-    for (int g = 0; g < VF_GROUPS; ++g) {
-      if (found) break;
-      double inc = (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      double cum = __shfl_up_sync(0xffffffffu, inc, 1);
+    for (int g = 0; g < GROUPS; ++g) {
+      double cum = __shfl_up_sync(0xffffffffu, inc[g], 1);
       cum = run + (lane > 0 ? cum : 0.0);
       int hit = -1, pos = -1;
 #pragma unroll
@@ -482,14 +490,14 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
           if (hit < 0 && cum > at) hit = pos;
         }
       }
-      const unsigned some = __ballot_sync(0xffffffffu, pos >= 0);
-      if (some) next = __shfl_sync(0xffffffffu, pos, 31 - __clz(some));
       const unsigned any = __ballot_sync(0xffffffffu, hit >= 0);
-      if (any) {
-        next = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
-        found = true;
+      const unsigned some = __ballot_sync(0xffffffffu, pos >= 0);
+      if (!found) {   // the first hit, or so far the last positive element
+        if (any) next = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
+        else if (some) next = __shfl_sync(0xffffffffu, pos, 31 - __clz(some));
+        found = any != 0;
       }
-      run += __shfl_sync(0xffffffffu, inc, 31);
+      run += __shfl_sync(0xffffffffu, inc[g], 31);
     }
     if (found) break;
   }
@@ -524,16 +532,20 @@ int verify_launch(const VerifyArgs& a, int max_q, cudaStream_t st) {
     return arg_err("draft_probs and draft_rows go together");
   if (a.draft_probs != nullptr && (a.ld_d < a.vocab || a.n_draft_rows < 0))
     return arg_err("draft_probs shape");
-  // few sequences: wide CTAs, two loads in flight cover a segment; many: one
-  // wave of smaller ones
+  // few sequences: clusters of 16 (a sequence on 16 SMs); many: smaller CTAs, four an SM, in
+  // one wave
   const int n = a.t.n_seqs;
   if (n > 0x7fffffff / VF_MAX_CLUSTER) return arg_err("n_seqs");
-  int cluster = 8;
-  if (n * 8 <= 148)
-    return launch_pdl(verify_kernel<512, 1>, dim3(n * cluster), dim3(512), 0, st, cluster,
+  if (n * 16 <= 148) {
+    static std::atomic<unsigned long long> devs{0};
+    if (int rc = wide_cluster_once(verify_kernel<512, 1, 5>, devs, "verification cluster attribute"))
+      return rc;
+    return launch_pdl(verify_kernel<512, 1, 5>, dim3(n * 16), dim3(512), 0, st, 16,
                       "draft verification launch", a);
-  while (cluster > 1 && n * (long long)cluster > 148 * 3) cluster /= 2;
-  return launch_pdl(verify_kernel<256, 3>, dim3(n * cluster), dim3(256), 0, st, cluster,
+  }
+  int cluster = 8;
+  while (cluster > 1 && n * (long long)cluster > 148 * 4) cluster /= 2;
+  return launch_pdl(verify_kernel<256, 4, 2>, dim3(n * cluster), dim3(256), 0, st, cluster,
                     "draft verification launch", a);
 }
 
