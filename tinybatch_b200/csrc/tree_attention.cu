@@ -150,11 +150,13 @@ static int tree_simple_launch(const TreeAttnArgs& t, cudaStream_t st) {
 // run on tcgen05 (M = 128 rows, tiles of 64 keys) with S, P and O in TMEM:
 //   warps 0-3  softmax: one query row a thread (TMEM lane = row); warps whose
 //              rows do not exist stay out
-//   warp 4     TMA: every 16 tokens one box {64 columns, 8 tokens, halves, K/V,
-//              2} of a 5-d view of the pool, i.e. K and V of a block and head in
-//              one request (8 KiB at hd 128).  It lands as [8-token group][K, V]
-//              [half][8][128 B], 128-byte swizzled, so K is a K-major operand and
-//              V an MN-major one whose 8-token groups lie 2 * halves KiB apart
+//   warp 4     TMA: every 16 tokens of K, and of V, one box {64 columns, 8 tokens,
+//              halves, 2} of a 4-d view of the pool (4 KiB at hd 128: all that
+//              a block keeps contiguous).  It lands as [8-token group][half][8]
+//              [128 B], 128-byte swizzled: K is a K-major operand and V an
+//              MN-major one, both with 8-token groups `halves` KiB apart.  K and
+//              V have rings of their own: a K stage is free once its S is done,
+//              two tiles before the V that came with it
 //   warp 5     MMA issue: S of the next tile goes into the other S buffer while
 //              the softmax works on this one; P (bf16) overwrites S in place and
 //              is read from TMEM
@@ -184,15 +186,16 @@ struct TreeTcLayout {
   static constexpr int HALVES = HD / 64;
   static constexpr int Q_HALF = TT_ROWS * 128;
   static constexpr int Q_TILE = HALVES * Q_HALF;
-  static constexpr int GROUP = 2 * HALVES * 1024;      // 8 tokens: K halves, V halves
+  static constexpr int GROUP = HALVES * 1024;          // 8 tokens of K (or V)
   static constexpr int BOX = 2 * GROUP;                // 16 tokens
   static constexpr int STAGE = TT_KEYS / 16 * BOX;
-  static constexpr int STAGES = HD == 128 ? 2 : 4;
-  static constexpr int OFF_KV = Q_TILE;
+  static constexpr int STAGES = HD == 128 ? 2 : 4;     // of K and of V
+  static constexpr int OFF_K = Q_TILE;
+  static constexpr int OFF_V = OFF_K + STAGES * STAGE;
   static constexpr int LDO = HD + 4;                   // floats a merged row (conflict-free float4 rows)
-  static constexpr int OFF_ML = OFF_KV + STAGES * STAGE;
+  static constexpr int OFF_ML = OFF_V + STAGES * STAGE;
   static constexpr int OFF_BAR = OFF_ML + TT_ROWS * 8;
-  static constexpr int N_BARS = 2 * STAGES + 7;
+  static constexpr int N_BARS = 4 * STAGES + 7;
   static constexpr int SMEM = OFF_BAR + 32 * 8 + 1024;
   static constexpr uint32_t COL_O = 2 * TT_KEYS;
   static constexpr uint32_t TMEM_COLS = 256;
@@ -202,12 +205,12 @@ struct TreeTcLayout {
   static_assert(2 * TT_KEYS + HD <= 256, "TMEM: two S buffers and O in half of it");
 };
 
-__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar,
-                                            int x4) {
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int x3) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %3, %3, %3, %4}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(x4)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %3, %3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(x3)
       : "memory");
 }
 
@@ -292,9 +295,11 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
   float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);   // [STAGES]
-  uint64_t* empty = full + L::STAGES;                               // [STAGES]
-  uint64_t* s_full = empty + L::STAGES;                             // [2]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR); // [STAGES]
+  uint64_t* k_empty = k_full + L::STAGES;                           // [STAGES]
+  uint64_t* v_full = k_empty + L::STAGES;                           // [STAGES]
+  uint64_t* v_empty = v_full + L::STAGES;                           // [STAGES]
+  uint64_t* s_full = v_empty + L::STAGES;                           // [2]
   uint64_t* p_full = s_full + 2;                                    // [2]
   uint64_t* pv_done = p_full + 2;                                   // [2]
   uint64_t* q_full = pv_done + 2;
@@ -331,8 +336,10 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   const int nt = (int)((long long)tiles * (rank + 1) / C) - t0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::STAGES; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -354,33 +361,38 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   unsigned long long m[TREE_WORDS] = {0, 0, 0, 0};
 
   if (warp == 4) {
-    // ---------------- loader
-    int ids = 0;
-    for (int j = 0; j < nt; ++j) {
+    // ---------------- loader: K of tile j + 1, then V of tile j (the order in which
+    // their stages come free)
+    int kid = 0, vid = 0;    // lane i: block of chunk i of the current eight tiles of K, of V
+    auto load = [&](int j, bool is_v, int& ids) -> bool {
       const int st = j % L::STAGES;
       const int c0 = (t0 + j) * (TT_KEYS / 16);
-      if (j % 8 == 0) {      // lane i: block of chunk c0 + i, for eight tiles
-        const int c = c0 + lane;
-        if (c < n_chunks) {
-          ids = table[c * 16 / a.block_size];
-          if (ids < 0 || ids >= a.num_blocks) {
-            set_status(ERR_BAD_INDEX);
-            ids = 0;         // load something valid; the result is flagged
-          }
+      if (j % 8 == 0 && c0 + lane < n_chunks) {
+        ids = table[(c0 + lane) * 16 / a.block_size];
+        if (ids < 0 || ids >= a.num_blocks) {
+          set_status(ERR_BAD_INDEX);
+          ids = 0;         // load something valid; the result is flagged
         }
       }
+      uint64_t* empty = is_v ? v_empty : k_empty;
+      uint64_t* full = (is_v ? v_full : k_full) + st;
       if (j >= L::STAGES &&
           !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / L::STAGES) - 1) & 1)))
-        break;
+        return false;
       const int nb = min(TT_KEYS / 16, n_chunks - c0);
       const int blk = __shfl_sync(0xffffffffu, ids, ((j % 8) * 4 + lane) & 31);
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], nb * L::BOX);
+      if (lane == 0) mbar_arrive_expect_tx(full, nb * L::BOX);
       __syncwarp();
       if (lane < nb) {
         const int slot = (c0 + lane) * 16 % a.block_size;
-        tma_load_5d(smem + L::OFF_KV + st * L::STAGE + lane * L::BOX, &map, &full[st],
-                    ((blk * 2 * a.n_kv_heads + kvh) * a.block_size + slot) / 8);
+        tma_load_4d(smem + (is_v ? L::OFF_V : L::OFF_K) + st * L::STAGE + lane * L::BOX, &map, full,
+                    (((blk * 2 + is_v) * a.n_kv_heads + kvh) * a.block_size + slot) / 8);
       }
+      return true;
+    };
+    for (int j = -1; j < nt; ++j) {
+      if (j + 1 < nt && !load(j + 1, false, kid)) break;
+      if (j >= 0 && !load(j, true, vid)) break;
     }
   } else if (warp == 5) {
     // ---------------- MMA issue
@@ -389,9 +401,9 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       constexpr uint32_t idesc_o = idesc_bf16_m128(HD) | (1u << 16);   // V: MN-major
       auto issue_s = [&](int j) -> bool {
         const int st = j % L::STAGES;
-        if (!mbar_wait(&full[st], (j / L::STAGES) & 1)) return false;
+        if (!mbar_wait(&k_full[st], (j / L::STAGES) & 1)) return false;
         tc_fence_after();
-        const uint32_t kb = sbase + L::OFF_KV + st * L::STAGE;
+        const uint32_t kb = sbase + L::OFF_K + st * L::STAGE;
 #pragma unroll
         for (int h = 0; h < L::HALVES; ++h)
 #pragma unroll
@@ -400,6 +412,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
                         sw128_k_desc(kb + h * 1024 + kk * 32, L::GROUP), idesc_s,
                         (h | kk) ? 1u : 0u);
         tc_commit(&s_full[j & 1]);
+        tc_commit(&k_empty[st]);
         return true;
       };
       bool good = mbar_wait(q_full, 0);
@@ -412,16 +425,17 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
           if (good) good = issue_s(j + 1);
           if (!good) break;
         }
+        const int st = j % L::STAGES;
+        if (!mbar_wait(&v_full[st], (j / L::STAGES) & 1)) break;
         if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1)) break;
         tc_fence_after();
-        const int st = j % L::STAGES;
-        const uint32_t vb = sbase + L::OFF_KV + st * L::STAGE + L::HALVES * 1024;
+        const uint32_t vb = sbase + L::OFF_V + st * L::STAGE;
 #pragma unroll
         for (int ks = 0; ks < TT_KEYS / 16; ++ks)
           tc_mma_bf16_ts(tmem + L::COL_O, tmem + (j & 1) * TT_KEYS + ks * 8,
                          sw128_mn_desc(vb + ks * 2 * L::GROUP, 1024, L::GROUP), idesc_o,
                          (j | ks) ? 1u : 0u);
-        tc_commit(&empty[st]);
+        tc_commit(&v_empty[st]);
         tc_commit(&pv_done[j & 1]);
       }
     }
@@ -476,8 +490,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
           if (!(wh & (1u << e))) x[32 + e] = -INFINITY;
         }
         const int st = j % L::STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (j / L::STAGES) & 1))) break;
-        uint8_t* vb = smem + L::OFF_KV + st * L::STAGE + L::HALVES * 1024;
+        if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / L::STAGES) & 1))) break;
+        uint8_t* vb = smem + L::OFF_V + st * L::STAGE;
         const int first = max(s.base - k0, 0);
         for (int i = first * (HD / 8) + r; i < TT_KEYS * (HD / 8); i += 32 * act) {
           const int key = i / (HD / 8), c = i % (HD / 8);
@@ -637,9 +651,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   }
 }
 
-// The pool as {64 columns, 8 tokens, halves, K/V, 8-token groups}: group g of
-// (block, K, head) starts at ((block * 2) * n_kv + head) * bs / 8 + g, its V one
-// K/V stride further.
+// The pool as {64 columns, 8 tokens, halves, 8-token groups}: group g of (block,
+// K or V, head) is number ((block * 2 + V) * n_kv + head) * bs / 8 + g.
 template <int HD>
 static int tree_pool_map(CUtensorMap* map, const AttnArgs& a) {
   EncodeTiledFn fn = encode_fn();
@@ -647,12 +660,12 @@ static int tree_pool_map(CUtensorMap* map, const AttnArgs& a) {
     set_last_error("cuTensorMapEncodeTiled entry point unavailable");
     return TB_ERR_CUDA;
   }
-  const cuuint64_t per_kv = (cuuint64_t)a.n_kv_heads * a.block_size;   // tokens between K and V
-  const cuuint64_t dims[5] = {64, 8, HD / 64, 2, ((cuuint64_t)a.num_blocks * 2 - 1) * per_kv / 8};
-  const cuuint64_t strides[4] = {HD * 2, 128, per_kv * HD * 2, 8 * HD * 2};
-  const cuuint32_t box[5] = {64, 8, HD / 64, 2, 2};
-  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<__nv_bfloat16*>(a.pool),
+  const cuuint64_t tokens = (cuuint64_t)a.num_blocks * 2 * a.n_kv_heads * a.block_size;
+  const cuuint64_t dims[4] = {64, 8, HD / 64, tokens / 8};
+  const cuuint64_t strides[3] = {HD * 2, 128, 8 * HD * 2};
+  const cuuint32_t box[4] = {64, 8, HD / 64, 2};
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16*>(a.pool),
                         dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
