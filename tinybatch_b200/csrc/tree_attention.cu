@@ -363,15 +363,25 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   if (warp == 4) {
     // ---------------- loader: K of tile j + 1, then V of tile j (the order in which
     // their stages come free)
-    int kid = 0, vid = 0;    // lane i: block of chunk i of the current eight tiles of K, of V
-    auto load = [&](int j, bool is_v, int& ids) -> bool {
+    // lane i: block of chunk i of the current eight tiles of K, of V, and of the next eight
+    auto blocks = [&](int j) -> int {
+      const int c = (t0 + j) * (TT_KEYS / 16) + lane;
+      if (c >= n_chunks) return 0;
+      const int id = table[c * 16 / a.block_size];
+      if (id >= 0 && id < a.num_blocks) return id;
+      set_status(ERR_BAD_INDEX);
+      return 0;            // load something valid; the result is flagged
+    };
+    int kid = 0, vid = 0, next = blocks(0);
+    auto load = [&](int j, bool is_v) -> bool {
       const int st = j % L::STAGES;
       const int c0 = (t0 + j) * (TT_KEYS / 16);
-      if (j % 8 == 0 && c0 + lane < n_chunks) {
-        ids = table[(c0 + lane) * 16 / a.block_size];
-        if (ids < 0 || ids >= a.num_blocks) {
-          set_status(ERR_BAD_INDEX);
-          ids = 0;         // load something valid; the result is flagged
+      if (j % 8 == 0) {
+        if (is_v) {
+          vid = kid;       // K is one tile ahead
+        } else {
+          kid = next;
+          next = blocks(j + 8);
         }
       }
       uint64_t* empty = is_v ? v_empty : k_empty;
@@ -380,7 +390,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
           !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / L::STAGES) - 1) & 1)))
         return false;
       const int nb = min(TT_KEYS / 16, n_chunks - c0);
-      const int blk = __shfl_sync(0xffffffffu, ids, ((j % 8) * 4 + lane) & 31);
+      const int blk = __shfl_sync(0xffffffffu, is_v ? vid : kid, ((j % 8) * 4 + lane) & 31);
       if (lane == 0) mbar_arrive_expect_tx(full, nb * L::BOX);
       __syncwarp();
       if (lane < nb) {
@@ -391,8 +401,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       return true;
     };
     for (int j = -1; j < nt; ++j) {
-      if (j + 1 < nt && !load(j + 1, false, kid)) break;
-      if (j >= 0 && !load(j, true, vid)) break;
+      if (j + 1 < nt && !load(j + 1, false)) break;
+      if (j >= 0 && !load(j, true)) break;
     }
   } else if (warp == 5) {
     // ---------------- MMA issue
@@ -450,23 +460,19 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     for (int i = 0; i < TREE_WORDS; ++i)
       if (i < t.mask_w && valid) m[i] = t.mask[row * t.mask_ld + i];
     {
-      // the warp's 32 rows, HD/8 lanes a row; missing rows are zero
+      // the warp's 32 rows, HD/8 lanes a row, straight into shared memory; missing rows are zero
       constexpr int PPR = HD / 8, RPI = 32 / PPR;
-      const unsigned long long mine =
-          valid ? row * a.ld_q + (size_t)(kvh * G + R % G) * HD : ~0ull;
-      uint4 v[32 / RPI];
+      const unsigned long long mine = row * a.ld_q + (size_t)(kvh * G + R % G) * HD;
+      const int c = lane % PPR;
 #pragma unroll
       for (int i = 0; i < 32 / RPI; ++i) {
-        const unsigned long long off = __shfl_sync(0xffffffffu, mine, i * RPI + lane / PPR);
-        v[i] = off != ~0ull ? *reinterpret_cast<const uint4*>(a.q + off + (lane % PPR) * 8)
-                            : make_uint4(0u, 0u, 0u, 0u);
+        const int rr = i * RPI + lane / PPR;
+        const unsigned long long off = __shfl_sync(0xffffffffu, mine, rr);
+        cp_async16(sbase + (c >> 3) * L::Q_HALF + sw128_off(warp * 32 + rr, c & 7),
+                   a.q + off + c * 8, warp * 32 + rr < nrows);
       }
-#pragma unroll
-      for (int i = 0; i < 32 / RPI; ++i) {
-        const int c = lane % PPR;
-        *reinterpret_cast<uint4*>(smem + (c >> 3) * L::Q_HALF +
-                                  sw128_off(warp * 32 + i * RPI + lane / PPR, c & 7)) = v[i];
-      }
+      cp_commit();
+      cp_wait<0>();
       fence_proxy_async_smem();
       mbar_arrive(q_full);
     }
