@@ -40,12 +40,12 @@ __device__ __forceinline__ bool tree_seq(const TreeAttnArgs& t, int seq, TreeSeq
          (int)(((long long)s.ctx + t.a.block_size - 1) / t.a.block_size) <= t.bt_w;
 }
 
-// ------------------------------------------------------------ any shape
+// ------------------------------------------------------------ short heads
 //
 // One warp a query row: lanes over keys for the scores (32 at a time, the row
 // of q broadcast from shared memory), over the head's columns for P V, both in
-// fp32 FMA, online softmax in base 2.  Serves the shapes the tensor-core kernel
-// below does not (head_dim 16, blocks that are no multiple of 16 tokens).
+// fp32 FMA, online softmax in base 2.  Serves head_dim 16, whose rows are too
+// short for the tensor-core kernel below.
 constexpr int TS_WARPS = 4;
 
 template <int HD>
@@ -146,25 +146,26 @@ static int tree_simple_launch(const TreeAttnArgs& t, cudaStream_t st) {
 // -------------------------------------------------------------- tensor cores
 //
 // One CTA per (row tile of 128 query rows, kv head, sequence) and split of its
-// context; the splits of a row tile form a cluster of C CTAs (1 to 8).  S = Q K^T and O += P V
-// run on tcgen05 (M = 128 rows, tiles of 64 keys) with S, P and O in TMEM:
+// context; the splits of a row tile form a cluster of C CTAs (1 to 8).  S = Q K^T
+// and O += P V run on tcgen05 (M = 128 rows, tiles of 64 keys) with S, P and O in
+// TMEM:
 //   warps 0-3  softmax: one query row a thread (TMEM lane = row); warps whose
 //              rows do not exist stay out
-//   warp 4     TMA: every 16 tokens of K, and of V, one box {64 columns, 8 tokens,
-//              halves, 2} of a 4-d view of the pool (4 KiB at hd 128: all that
-//              a block keeps contiguous).  It lands as [8-token group][half][8]
-//              [128 B], 128-byte swizzled: K is a K-major operand and V an
-//              MN-major one, both with 8-token groups `halves` KiB apart.  K and
-//              V have rings of their own: a K stage is free once its S is done,
-//              two tiles before the V that came with it
+//   warp 4     loads.  Block sizes that are multiples of 16: every 16 tokens of K,
+//              and of V, are one TMA box {64 columns, 8 tokens, halves, 2} of a 4-d
+//              view of the pool (4 KiB at hd 128, all that a block keeps
+//              contiguous), landing as [8-token group][half][8][128 B] with the
+//              128-byte swizzle: K is a K-major operand and V an MN-major one.  Four
+//              lanes issue a tile's boxes.  Other block sizes: 16-byte cp.async pieces into the same layout, every key looking up its
+//              block (a third slower).  K and V have rings of their own: a K stage
+//              is free once its S is done, before the V that came with it
 //   warp 5     MMA issue: S of the next tile goes into the other S buffer while
 //              the softmax works on this one; P (bf16) overwrites S in place and
 //              is read from TMEM
 // O is accumulated in TMEM; a row's exponent reference moves only when its
 // maximum has grown by more than TT_RESCALE (log2 units), as in the prefill kernel.
-// A quarter of an SM's shared memory would hold fewer keys in flight than HBM's
-// latency asks for, half of it with two CTAs an SM hides one CTA's chain S ->
-// softmax -> P V, its start and its end behind the other's loads.
+// Two CTAs an SM: one's chain S -> softmax -> P V, its start and its end hide
+// behind the other's loads.
 //
 // Tiles that hold drafts (or places past the context) apply the mask to S and
 // clean V in shared memory before P V: rows past the context become zero (a
@@ -188,18 +189,19 @@ struct TreeTcLayout {
   static constexpr int Q_TILE = HALVES * Q_HALF;
   static constexpr int GROUP = HALVES * 1024;          // 8 tokens of K (or V)
   static constexpr int BOX = 2 * GROUP;                // 16 tokens
-  static constexpr int STAGE = TT_KEYS / 16 * BOX;
+  static constexpr int STAGE = TT_KEYS / 8 * GROUP;
   static constexpr int STAGES = HD == 128 ? 2 : 4;     // of K and of V
   static constexpr int OFF_K = Q_TILE;
   static constexpr int OFF_V = OFF_K + STAGES * STAGE;
   static constexpr int LDO = HD + 4;                   // floats a merged row (conflict-free float4 rows)
+  static constexpr int OFF_W = TT_ROWS * LDO * 4;      // merge weights [row][split], behind the rows
   static constexpr int OFF_ML = OFF_V + STAGES * STAGE;
   static constexpr int OFF_BAR = OFF_ML + TT_ROWS * 8;
   static constexpr int N_BARS = 4 * STAGES + 7;
   static constexpr int SMEM = OFF_BAR + 32 * 8 + 1024;
   static constexpr uint32_t COL_O = 2 * TT_KEYS;
   static constexpr uint32_t TMEM_COLS = 256;
-  static_assert(TT_ROWS * LDO * 4 <= OFF_ML, "merge rows over Q and the ring");
+  static_assert(OFF_W + TT_ROWS * TT_MAX_SPLITS * 4 <= OFF_ML, "merge rows and weights over Q and the rings");
   static_assert(N_BARS * 8 + 8 <= 32 * 8, "barrier area");
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
   static_assert(2 * TT_KEYS + HD <= 256, "TMEM: two S buffers and O in half of it");
@@ -287,7 +289,7 @@ __device__ __forceinline__ void for_nonfinite(const TreeAttnArgs& t, const int* 
   }
 }
 
-template <int HD>
+template <int HD, bool TMA>
 __global__ void __launch_bounds__(TT_THREADS, 2)
     tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map, const TreeAttnArgs t,
                         const int row_tiles) {
@@ -311,11 +313,27 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   const int kvh = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles;
   const int seq = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t sbase = smem_u32(smem);
   if (warp == 5) {
     tmem_alloc(tmem_slot, L::TMEM_COLS);
     tmem_relinquish();
+  } else if (warp == 4) {
+    if (lane == 0) {
+      for (int i = 0; i < L::STAGES; ++i) {
+        mbar_init(&k_full[i], TMA ? 1 : 32);
+        mbar_init(&k_empty[i], 1);
+        mbar_init(&v_full[i], TMA ? 1 : 32);
+        mbar_init(&v_empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&pv_done[i], 1);
+      }
+      fence_mbar_init();
+      if (TMA) prefetch_tmap(&map);
+    }
+    __syncwarp();
   }
-  if (threadIdx.x == 0) prefetch_tmap(&map);
   pdl_wait();
   TreeSeq s;
   const bool ok = tree_seq(t, seq, s);
@@ -330,22 +348,90 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   const int nrows = min(rows, TT_ROWS);
   const int act = (nrows + 31) / 32;               // softmax warps with rows
   const int* table = a.block_tables + (size_t)seq * a.bt_ld;
-  const int n_chunks = (s.ctx + 15) / 16;
-  const int tiles = (s.ctx + TT_KEYS - 1) / TT_KEYS;
-  const int t0 = (int)((long long)tiles * rank / C);
-  const int nt = (int)((long long)tiles * (rank + 1) / C) - t0;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < L::STAGES; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+  const unsigned tiles = (unsigned)(s.ctx + TT_KEYS - 1) / TT_KEYS;   // (below 2^26: times C fits)
+  const int t0 = (int)(tiles * rank / C);
+  const int nt = (int)(tiles * (rank + 1) / C) - t0;
+
+  // ---- loader state (warp 4)
+  // TMA: lane i holds the 8-token group of K of chunk i (16 tokens) of eight tiles
+  int kid = 0, vid = 0, next = 0;
+  auto chunks = [&](int j) -> int {
+    const int c = t0 * (TT_KEYS / 16) + j * (TT_KEYS / 16) + lane;
+    if (c * 16 >= s.ctx) return 0;
+    int blk = table[c * 16 / a.block_size];
+    if (blk < 0 || blk >= a.num_blocks) {
+      set_status(ERR_BAD_INDEX);
+      blk = 0;             // load something valid; the result is flagged
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 32 * act);
-      mbar_init(&pv_done[i], 1);
+    return (blk * 2 * a.n_kv_heads + kvh) * (a.block_size / 8) + c * 16 % a.block_size / 8;
+  };
+  const int v_off = a.n_kv_heads * (a.block_size / 8);   // from K's group to V's
+  auto issue = [&](int j, bool is_v) {
+    const int st = j & (L::STAGES - 1);
+    const int g = __shfl_sync(0xffffffffu, is_v ? vid : kid, ((j & 7) * 4 + lane) & 31);
+    const int left = (s.ctx - (t0 + j) * TT_KEYS + 15) / 16;   // boxes of the tile
+    uint64_t* full = (is_v ? v_full : k_full) + st;
+    if (lane == 0) mbar_arrive_expect_tx(full, min(left, TT_KEYS / 16) * L::BOX);
+    __syncwarp();
+    if (lane < min(left, TT_KEYS / 16))
+      tma_load_4d(smem + (is_v ? L::OFF_V : L::OFF_K) + st * L::STAGE + lane * L::BOX, &map, full,
+                  is_v ? g + v_off : g);
+  };
+  // cp.async: pool rows (of hd elements) of keys lane and lane + 32 of a tile
+  unsigned krow[2], vrow[2], nrow[2] = {0, 0};
+  auto find = [&](int j, unsigned* row) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int p = (t0 + j) * TT_KEYS + 32 * h + lane;
+      row[h] = ~0u;        // past the context: zeros
+      if (p < s.ctx) {
+        const int blk = table[p / a.block_size];
+        if (blk >= 0 && blk < a.num_blocks)
+          row[h] = ((unsigned)blk * 2 * a.n_kv_heads + kvh) * a.block_size + p % a.block_size;
+        else
+          set_status(ERR_BAD_INDEX);
+      }
     }
+  };
+  auto copy = [&](int j, const unsigned* row, bool is_v) {
+    constexpr int PPR = HD / 8, RPI = 32 / PPR;    // lanes a row, rows an instruction
+    const uint32_t st = sbase + (is_v ? L::OFF_V : L::OFF_K) + (j % L::STAGES) * L::STAGE;
+    const int c = lane % PPR;
+    const __nv_bfloat16* src =
+        a.pool + c * 8 + (is_v ? (size_t)a.n_kv_heads * a.block_size * HD : 0);
+#pragma unroll
+    for (int i = 0; i < TT_KEYS / RPI; ++i) {
+      const int key = i * RPI + lane / PPR;
+      const unsigned r = __shfl_sync(0xffffffffu, row[i * RPI / 32], key & 31);
+      cp_async16(st + (key >> 3) * L::GROUP + (c >> 3) * 1024 + sw128_off(key & 7, c & 7),
+                 src + (r != ~0u ? (size_t)r * HD : 0), r != ~0u);
+    }
+    cp_arrive_noinc((is_v ? v_full : k_full) + j % L::STAGES);
+  };
+  // ---- softmax warps: the queries of the warp's 32 rows go straight to shared
+  // memory (HD/8 lanes a row; missing rows are zero) while the CTA meets
+  const int r = threadIdx.x;                       // row of a softmax thread
+  const bool valid = r < nrows;
+  const int R = rt * TT_ROWS + (valid ? r : 0);
+  const size_t row = (size_t)s.q0 + R / G;
+  unsigned long long m[TREE_WORDS] = {0, 0, 0, 0};
+  if (warp < act) {
+    constexpr int PPR = HD / 8, RPI = 32 / PPR;
+    const unsigned long long mine = row * a.ld_q + (size_t)(kvh * G + R % G) * HD;
+    const int c = lane % PPR;
+#pragma unroll
+    for (int i = 0; i < 32 / RPI; ++i) {
+      const int rr = i * RPI + lane / PPR;
+      const unsigned long long off = __shfl_sync(0xffffffffu, mine, rr);
+      cp_async16(sbase + (c >> 3) * L::Q_HALF + sw128_off(warp * 32 + rr, c & 7),
+                 a.q + off + c * 8, warp * 32 + rr < nrows);
+    }
+    cp_commit();
+#pragma unroll
+    for (int i = 0; i < TREE_WORDS; ++i)
+      if (i < t.mask_w && valid) m[i] = t.mask[row * t.mask_ld + i];
+  } else if (warp == 4 && lane == 0) {
+    for (int i = 0; i < 2; ++i) mbar_init(&p_full[i], 32 * act);
     mbar_init(q_full, 32 * act);
     *s_bad = 0;
     fence_mbar_init();
@@ -356,53 +442,59 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   // only now: a dependent kernel that takes tensor memory must not get in before this CTA's
   if (threadIdx.x == 0) pdl_trigger();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t sbase = smem_u32(smem);
   float ref = -INFINITY, l = 0.f;                  // a row's exponent reference (log2) and sum
-  unsigned long long m[TREE_WORDS] = {0, 0, 0, 0};
 
   if (warp == 4) {
     // ---------------- loader: K of tile j + 1, then V of tile j (the order in which
-    // their stages come free)
-    // lane i: block of chunk i of the current eight tiles of K, of V, and of the next eight
-    auto blocks = [&](int j) -> int {
-      const int c = (t0 + j) * (TT_KEYS / 16) + lane;
-      if (c >= n_chunks) return 0;
-      const int id = table[c * 16 / a.block_size];
-      if (id >= 0 && id < a.num_blocks) return id;
-      set_status(ERR_BAD_INDEX);
-      return 0;            // load something valid; the result is flagged
-    };
-    int kid = 0, vid = 0, next = blocks(0);
-    auto load = [&](int j, bool is_v) -> bool {
-      const int st = j % L::STAGES;
-      const int c0 = (t0 + j) * (TT_KEYS / 16);
-      if (j % 8 == 0) {
-        if (is_v) {
-          vid = kid;       // K is one tile ahead
-        } else {
+    // their stages come free); block ids are read a window or a tile ahead
+    if (TMA) {
+      if (nt > 0) {
+        kid = chunks(0);
+        issue(0, false);
+      }
+      next = chunks(8);
+      for (int j = 0; j < nt; ++j) {
+        vid = kid;
+        if (((j + 1) & 7) == 0) {
           kid = next;
-          next = blocks(j + 8);
+          next = chunks(j + 9);
         }
+        if (j + 1 < nt) {
+          if (j + 1 >= L::STAGES &&
+              !__all_sync(0xffffffffu, mbar_wait(&k_empty[(j + 1) & (L::STAGES - 1)],
+                                                 ((j + 1) / L::STAGES - 1) & 1)))
+            break;
+          issue(j + 1, false);
+        }
+        if (j >= L::STAGES &&
+            !__all_sync(0xffffffffu, mbar_wait(&v_empty[j & (L::STAGES - 1)],
+                                               (j / L::STAGES - 1) & 1)))
+          break;
+        issue(j, true);
       }
-      uint64_t* empty = is_v ? v_empty : k_empty;
-      uint64_t* full = (is_v ? v_full : k_full) + st;
-      if (j >= L::STAGES &&
-          !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / L::STAGES) - 1) & 1)))
-        return false;
-      const int nb = min(TT_KEYS / 16, n_chunks - c0);
-      const int blk = __shfl_sync(0xffffffffu, is_v ? vid : kid, ((j % 8) * 4 + lane) & 31);
-      if (lane == 0) mbar_arrive_expect_tx(full, nb * L::BOX);
-      __syncwarp();
-      if (lane < nb) {
-        const int slot = (c0 + lane) * 16 % a.block_size;
-        tma_load_4d(smem + (is_v ? L::OFF_V : L::OFF_K) + st * L::STAGE + lane * L::BOX, &map, full,
-                    (((blk * 2 + is_v) * a.n_kv_heads + kvh) * a.block_size + slot) / 8);
+    } else {
+      if (nt > 0) {
+        find(0, krow);
+        copy(0, krow, false);
       }
-      return true;
-    };
-    for (int j = -1; j < nt; ++j) {
-      if (j + 1 < nt && !load(j + 1, false)) break;
-      if (j >= 0 && !load(j, true)) break;
+      if (nt > 1) find(1, nrow);
+      for (int j = 0; j < nt; ++j) {
+        vrow[0] = krow[0], vrow[1] = krow[1];
+        if (j + 1 < nt) {
+          krow[0] = nrow[0], krow[1] = nrow[1];
+          if (j + 2 < nt) find(j + 2, nrow);
+          if (j + 1 >= L::STAGES &&
+              !__all_sync(0xffffffffu, mbar_wait(&k_empty[(j + 1) % L::STAGES],
+                                                 ((j + 1) / L::STAGES - 1) & 1)))
+            break;
+          copy(j + 1, krow, false);
+        }
+        if (j >= L::STAGES &&
+            !__all_sync(0xffffffffu, mbar_wait(&v_empty[j % L::STAGES], (j / L::STAGES - 1) & 1)))
+          break;
+        copy(j, vrow, true);
+      }
+      cp_wait<0>();   // nothing in flight at exit
     }
   } else if (warp == 5) {
     // ---------------- MMA issue
@@ -413,6 +505,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
         const int st = j % L::STAGES;
         if (!mbar_wait(&k_full[st], (j / L::STAGES) & 1)) return false;
         tc_fence_after();
+        if (!TMA) fence_proxy_async_smem();   // K arrived through the generic proxy
         const uint32_t kb = sbase + L::OFF_K + st * L::STAGE;
 #pragma unroll
         for (int h = 0; h < L::HALVES; ++h)
@@ -439,6 +532,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
         if (!mbar_wait(&v_full[st], (j / L::STAGES) & 1)) break;
         if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1)) break;
         tc_fence_after();
+        if (!TMA) fence_proxy_async_smem();   // V too
         const uint32_t vb = sbase + L::OFF_V + st * L::STAGE;
 #pragma unroll
         for (int ks = 0; ks < TT_KEYS / 16; ++ks)
@@ -452,30 +546,9 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     __syncwarp();
   } else if (warp < act) {
     // ---------------- softmax: one row a thread
-    const int r = threadIdx.x;
-    const bool valid = r < nrows;
-    const int R = rt * TT_ROWS + (valid ? r : 0);
-    const size_t row = (size_t)s.q0 + R / G;
-#pragma unroll
-    for (int i = 0; i < TREE_WORDS; ++i)
-      if (i < t.mask_w && valid) m[i] = t.mask[row * t.mask_ld + i];
-    {
-      // the warp's 32 rows, HD/8 lanes a row, straight into shared memory; missing rows are zero
-      constexpr int PPR = HD / 8, RPI = 32 / PPR;
-      const unsigned long long mine = row * a.ld_q + (size_t)(kvh * G + R % G) * HD;
-      const int c = lane % PPR;
-#pragma unroll
-      for (int i = 0; i < 32 / RPI; ++i) {
-        const int rr = i * RPI + lane / PPR;
-        const unsigned long long off = __shfl_sync(0xffffffffu, mine, rr);
-        cp_async16(sbase + (c >> 3) * L::Q_HALF + sw128_off(warp * 32 + rr, c & 7),
-                   a.q + off + c * 8, warp * 32 + rr < nrows);
-      }
-      cp_commit();
-      cp_wait<0>();
-      fence_proxy_async_smem();
-      mbar_arrive(q_full);
-    }
+    cp_wait<0>();
+    fence_proxy_async_smem();
+    mbar_arrive(q_full);
     const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
     const uint32_t to = tmem + L::COL_O + lane_off;
     const float sc = a.scale_log2;
@@ -505,14 +578,14 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
                                               sw128_off(key & 7, c & 7));
           if (k0 + key >= s.ctx) {
             *p = make_uint4(0u, 0u, 0u, 0u);
-          } else {
-            uint4 q = *p;
-            const uint4 n = make_uint4(nonfinite2(q.x), nonfinite2(q.y), nonfinite2(q.z), nonfinite2(q.w));
-            if (n.x | n.y | n.z | n.w) {
-              q.x &= ~n.x, q.y &= ~n.y, q.z &= ~n.z, q.w &= ~n.w;
-              *p = q;
-              *s_bad = 1;
-            }
+            continue;
+          }
+          uint4 q = *p;
+          const uint4 n = make_uint4(nonfinite2(q.x), nonfinite2(q.y), nonfinite2(q.z), nonfinite2(q.w));
+          if (n.x | n.y | n.z | n.w) {
+            q.x &= ~n.x, q.y &= ~n.y, q.z &= ~n.z, q.w &= ~n.w;
+            *p = q;
+            *s_bad = 1;
           }
         }
         fence_proxy_async_smem();
@@ -572,13 +645,10 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   const int j1 = min((t0 + nt) * TT_KEYS - s.base, s.ql);
   const bool bad = *s_bad != 0;
   if (warp < act) {
-    const int r = threadIdx.x;
-    const bool valid = r < nrows;
-    const int R = rt * TT_ROWS + (valid ? r : 0);
     const uint32_t to = tmem + L::COL_O + ((uint32_t)(warp * 32) << 16);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     __nv_bfloat16* dst =
-        a.out + ((size_t)s.q0 + R / G) * a.ld_out + (size_t)(kvh * G + R % G) * HD;
+        a.out + row * a.ld_out + (size_t)(kvh * G + R % G) * HD;
     float* keep = reinterpret_cast<float*>(smem) + r * L::LDO;
 #pragma unroll
     for (int c0 = 0; c0 < HD; c0 += 32) {
@@ -602,7 +672,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     }
     if (C > 1) s_ml[r] = make_float2(ref, l);
     if (bad && valid)
-      for_nonfinite<HD>(t, table, kvh, (size_t)s.q0 + R / G, s.base, j0, j1, [&](int c, float x) {
+      for_nonfinite<HD>(t, table, kvh, row, s.base, j0, j1, [&](int c, float x) {
         if (C > 1) keep[c] += x;
         else dst[c] = __float2bfloat16_rn(__bfloat162float(dst[c]) + x);
       });
@@ -612,41 +682,75 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     __syncthreads();
   } else {
     cluster_sync_all();
-    // this CTA's 1/C of the rows: HD/4 lanes a row, four columns each
-    constexpr int LPR = HD / 4, RPW = 32 / LPR;
+    // this CTA's 1/C of the rows: each row's weights first, then its columns, four
+    // a lane, several remote loads in flight
     const int per = (nrows + C - 1) / C;
-    const int r1 = min((rank + 1) * per, nrows);
-    for (int rb = rank * per + warp * RPW; rb < r1; rb += (TT_THREADS / 32) * RPW) {
-      const int r = rb + lane / LPR;
-      const int rr = min(r, r1 - 1);
-      const int c = (lane % LPR) * 4;
+    const int r0 = min(rank * per, nrows), n = min(per, nrows - r0);
+    float* wt = reinterpret_cast<float*>(smem + L::OFF_W);
+    if (threadIdx.x < n) {
+      const int r = r0 + threadIdx.x;
       float2 ml[TT_MAX_SPLITS];
-      float M = -INFINITY;
+      float M = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int z = 0; z < TT_MAX_SPLITS; ++z)
+        if (z < C) ml[z] = ld_cluster_f2(cluster_map(sbase + L::OFF_ML + r * 8, z));
+#pragma unroll
+      for (int z = 0; z < TT_MAX_SPLITS; ++z)
+        if (z < C) M = fmaxf(M, ml[z].x);
+      const float mu = M == -INFINITY ? 0.f : M;
 #pragma unroll
       for (int z = 0; z < TT_MAX_SPLITS; ++z)
         if (z < C) {
-          ml[z] = ld_cluster_f2(cluster_map(sbase + L::OFF_ML + rr * 8, z));
-          M = fmaxf(M, ml[z].x);
-        }
-      const float mu = M == -INFINITY ? 0.f : M;
-      float sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int z = 0; z < TT_MAX_SPLITS; ++z)
-        if (z < C && !(ml[z].x == -INFINITY && ml[z].y == 0.f)) {   // a split that saw nothing
-          const float w = ex2_approx(ml[z].x - mu);
-          const float4 o = ld_cluster_f4(cluster_map(sbase + (rr * L::LDO + c) * 4, z));
-          sum += w * ml[z].y;
-          acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
+          ml[z].x = ex2_approx(ml[z].x - mu);      // 0 for a split that saw nothing
+          sum += ml[z].x * ml[z].y;
         }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      if (r < r1) {
-        const int R = rt * TT_ROWS + r;
-        uint2 u;
-        u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-        u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(a.out + ((size_t)s.q0 + R / G) * a.ld_out +
-                                  (size_t)(kvh * G + R % G) * HD + c) = u;
+#pragma unroll
+      for (int z = 0; z < TT_MAX_SPLITS; ++z)
+        if (z < C) wt[threadIdx.x * TT_MAX_SPLITS + z] = ml[z].x * inv;
+    }
+    __syncthreads();
+    constexpr int LPR = HD / 4, UN = 2;
+    const int items = n * LPR;
+    for (int i0 = threadIdx.x; i0 < items; i0 += UN * TT_THREADS) {
+      float4 acc[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int z0 = 0; z0 < TT_MAX_SPLITS; z0 += 4) {
+        if (z0 >= C) break;
+        float4 o[UN][4];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          const int i = min(i0 + u * TT_THREADS, items - 1);
+          const uint32_t src = sbase + ((r0 + i / LPR) * L::LDO + (i % LPR) * 4) * 4;
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+            if (z0 + z < C) o[u][z] = ld_cluster_f4(cluster_map(src, z0 + z));
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          const int i = min(i0 + u * TT_THREADS, items - 1);
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+            if (z0 + z < C) {
+              const float w = wt[i / LPR * TT_MAX_SPLITS + z0 + z];
+              acc[u].x += w * o[u][z].x, acc[u].y += w * o[u][z].y;
+              acc[u].z += w * o[u][z].z, acc[u].w += w * o[u][z].w;
+            }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int i = i0 + u * TT_THREADS;
+        if (i < items) {
+          const int R = rt * TT_ROWS + r0 + i / LPR;
+          uint2 v;
+          v.x = pack_bf16x2(acc[u].x, acc[u].y);
+          v.y = pack_bf16x2(acc[u].z, acc[u].w);
+          *reinterpret_cast<uint2*>(a.out + ((size_t)s.q0 + R / G) * a.ld_out +
+                                    (size_t)(kvh * G + R % G) * HD + (i % LPR) * 4) = v;
+        }
       }
     }
     cluster_sync_all();   // peers read this CTA's shared memory until here
@@ -693,20 +797,21 @@ static int tree_splits(int n_seqs, int n_kv, int row_tiles, int max_ctx, long lo
   return c >= 8 ? 8 : c >= 4 ? 4 : c >= 2 ? 2 : 1;
 }
 
-template <int HD>
+template <int HD, bool TMA>
 static int tree_tc_launch(const TreeAttnArgs& t, int max_ctx, long long ctx_total, cudaStream_t st) {
   using L = TreeTcLayout<HD>;
   static std::atomic<unsigned long long> attr_devs{0};
-  if (int rc = smem_attr_once(tree_attn_tc_kernel<HD>, L::SMEM, attr_devs,
+  if (int rc = smem_attr_once(tree_attn_tc_kernel<HD, TMA>, L::SMEM, attr_devs,
                               "tree attention smem attribute", true))
     return rc;
-  CUtensorMap map;
-  if (int rc = tree_pool_map<HD>(&map, t.a)) return rc;
+  CUtensorMap map{};
+  if (TMA)
+    if (int rc = tree_pool_map<HD>(&map, t.a)) return rc;
   const long long rows = (long long)t.max_q * (t.a.n_q_heads / t.a.n_kv_heads);
   const int row_tiles = (int)((rows + TT_ROWS - 1) / TT_ROWS);
   if ((long long)row_tiles * t.a.n_kv_heads > 65535) return arg_err("too many heads and nodes");
   const int C = tree_splits(t.a.n_seqs, t.a.n_kv_heads, row_tiles, max_ctx, ctx_total);
-  return launch_pdl(tree_attn_tc_kernel<HD>, dim3(C, t.a.n_kv_heads * row_tiles, t.a.n_seqs),
+  return launch_pdl(tree_attn_tc_kernel<HD, TMA>, dim3(C, t.a.n_kv_heads * row_tiles, t.a.n_seqs),
                     dim3(TT_THREADS), L::SMEM, st, C, "tree attention launch", map, t, row_tiles);
 }
 
@@ -739,13 +844,18 @@ int tree_attention(TreeAttnArgs t, int head_dim, int max_ctx, long long ctx_tota
   if (max_ctx <= 0 || max_ctx > width) max_ctx = (int)(width < 0x7fffffff ? width : 0x7fffffff);
   if (ctx_total <= 0 || ctx_total > (long long)max_ctx * a.n_seqs)
     ctx_total = (long long)max_ctx * a.n_seqs;
-  // 16-token boxes inside one block; the group index is a 32-bit coordinate
-  const bool tc = a.block_size % 16 == 0 &&
-                  (long long)a.num_blocks * 2 * a.n_kv_heads * a.block_size < (1ll << 31);
+  // pool rows (tokens of one head) are 32-bit numbers in the kernels
+  if ((long long)a.num_blocks * 2 * a.n_kv_heads * a.block_size >= 0xffffffffll)
+    return arg_err("KV pool rows beyond 2^32");
+  const bool tma = a.block_size % 16 == 0;      // 16-token boxes inside one block
   switch (head_dim) {
     case 16: return tree_simple_launch<16>(t, st);
-    case 64: return tc ? tree_tc_launch<64>(t, max_ctx, ctx_total, st) : tree_simple_launch<64>(t, st);
-    default: return tc ? tree_tc_launch<128>(t, max_ctx, ctx_total, st) : tree_simple_launch<128>(t, st);
+    case 64:
+      return tma ? tree_tc_launch<64, true>(t, max_ctx, ctx_total, st)
+                 : tree_tc_launch<64, false>(t, max_ctx, ctx_total, st);
+    default:
+      return tma ? tree_tc_launch<128, true>(t, max_ctx, ctx_total, st)
+                 : tree_tc_launch<128, false>(t, max_ctx, ctx_total, st);
   }
 }
 
