@@ -173,9 +173,9 @@ static int tree_simple_launch(const TreeAttnArgs& t, cudaStream_t st) {
 // elements of draft nodes, which the epilogue adds back to the rows that see
 // them.
 //
-// With C > 1 every CTA leaves (reference, sum, O) of its rows in its own shared
-// memory and each merges 1/C of the rows over the cluster, in split order: no
-// workspace, no counters, nothing shared between calls.
+// With C > 1 the CTAs of a cluster exchange (reference, sum, O) through their
+// shared memory and each merges 1/C of the rows, in split order: no workspace, no
+// counters, nothing shared between calls.
 constexpr int TT_ROWS = 128;
 constexpr int TT_KEYS = 64;
 constexpr int TT_THREADS = 192;
@@ -193,15 +193,14 @@ struct TreeTcLayout {
   static constexpr int STAGES = HD == 128 ? 2 : 4;     // of K and of V
   static constexpr int OFF_K = Q_TILE;
   static constexpr int OFF_V = OFF_K + STAGES * STAGE;
-  static constexpr int LDO = HD + 4;                   // floats a merged row (conflict-free float4 rows)
-  static constexpr int OFF_W = TT_ROWS * LDO * 4;      // merge weights [row][split], behind the rows
   static constexpr int OFF_ML = OFF_V + STAGES * STAGE;
-  static constexpr int OFF_BAR = OFF_ML + TT_ROWS * 8;
+  static constexpr int OFF_OUT = OFF_ML + (TT_ROWS + TT_MAX_SPLITS) * 8;   // rows' places in out
+  static constexpr int OFF_BAR = OFF_OUT + TT_ROWS * 8;
   static constexpr int N_BARS = 4 * STAGES + 7;
   static constexpr int SMEM = OFF_BAR + 32 * 8 + 1024;
   static constexpr uint32_t COL_O = 2 * TT_KEYS;
   static constexpr uint32_t TMEM_COLS = 256;
-  static_assert(OFF_W + TT_ROWS * TT_MAX_SPLITS * 4 <= OFF_ML, "merge rows and weights over Q and the rings");
+  static_assert((TT_ROWS + 2 * TT_MAX_SPLITS) * HD * 4 <= OFF_ML, "merged rows over Q and the rings");
   static_assert(N_BARS * 8 + 8 <= 32 * 8, "barrier area");
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
   static_assert(2 * TT_KEYS + HD <= 256, "TMEM: two S buffers and O in half of it");
@@ -222,18 +221,11 @@ __device__ __forceinline__ uint64_t sw128_k_desc(uint32_t smem_addr, uint32_t sb
          (uint64_t)1u << 46 | (uint64_t)2u << 61;
 }
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_f2(uint32_t addr, float x, float y) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(addr), "f"(x), "f"(y) : "memory");
 }
-__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t x) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
 }
 
 // Bits of a word whose bf16 halves are infinite or NaN (those halves all ones).
@@ -266,16 +258,16 @@ __device__ __forceinline__ unsigned long long tree_window(const unsigned long lo
   return w;
 }
 
-// For every non-finite value of the draft nodes j0 .. j1-1 that row `row` sees
-// (their products were left out of P V): add(column, value).
-template <int HD, class F>
-__device__ __forceinline__ void for_nonfinite(const TreeAttnArgs& t, const int* table, int kvh,
-                                              size_t row, int base, int j0, int j1, F add) {
+// Adds to a finished output row the non-finite values of the draft nodes it
+// sees (their products were left out of P V).  Rare.
+template <int HD>
+__device__ __forceinline__ void add_nonfinite(const TreeAttnArgs& t, const int* table, int kvh,
+                                              size_t row, const TreeSeq& s, __nv_bfloat16* dst) {
   const AttnArgs& a = t.a;
 #pragma unroll 1
-  for (int j = j0; j < j1; ++j) {
+  for (int j = 0; j < s.ql; ++j) {
     if (!((t.mask[row * t.mask_ld + (j >> 6)] >> (j & 63)) & 1)) continue;
-    const int p = base + j;
+    const int p = s.base + j;
     const int blk = table[p / a.block_size];
     if (blk < 0 || blk >= a.num_blocks) continue;
     const __nv_bfloat16* src =
@@ -284,7 +276,7 @@ __device__ __forceinline__ void for_nonfinite(const TreeAttnArgs& t, const int* 
 #pragma unroll 1
     for (int c = 0; c < HD; ++c) {
       const float x = __bfloat162float(src[c]);
-      if (!isfinite(x)) add(c, x);
+      if (!isfinite(x)) dst[c] = __float2bfloat16_rn(__bfloat162float(dst[c]) + x);
     }
   }
 }
@@ -297,6 +289,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
   float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
+  size_t* s_out = reinterpret_cast<size_t*>(smem + L::OFF_OUT);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR); // [STAGES]
   uint64_t* k_empty = k_full + L::STAGES;                           // [STAGES]
   uint64_t* v_full = k_empty + L::STAGES;                           // [STAGES]
@@ -335,6 +328,11 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     __syncwarp();
   }
   pdl_wait();
+  const int* table = a.block_tables + (size_t)seq * a.bt_ld;
+  // the first split starts at token 0: its block ids need not wait for the metadata
+  int early = 0;
+  if (TMA && warp == 4 && rank == 0 && lane * 16 / a.block_size < t.bt_w)
+    early = table[lane * 16 / a.block_size];
   TreeSeq s;
   const bool ok = tree_seq(t, seq, s);
   const int G = a.n_q_heads / a.n_kv_heads;
@@ -347,7 +345,6 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   }
   const int nrows = min(rows, TT_ROWS);
   const int act = (nrows + 31) / 32;               // softmax warps with rows
-  const int* table = a.block_tables + (size_t)seq * a.bt_ld;
   const unsigned tiles = (unsigned)(s.ctx + TT_KEYS - 1) / TT_KEYS;   // (below 2^26: times C fits)
   const int t0 = (int)(tiles * rank / C);
   const int nt = (int)(tiles * (rank + 1) / C) - t0;
@@ -355,10 +352,10 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   // ---- loader state (warp 4)
   // TMA: lane i holds the 8-token group of K of chunk i (16 tokens) of eight tiles
   int kid = 0, vid = 0, next = 0;
-  auto chunks = [&](int j) -> int {
+  auto chunks = [&](int j, bool have) -> int {
     const int c = t0 * (TT_KEYS / 16) + j * (TT_KEYS / 16) + lane;
     if (c * 16 >= s.ctx) return 0;
-    int blk = table[c * 16 / a.block_size];
+    int blk = have ? early : table[c * 16 / a.block_size];
     if (blk < 0 || blk >= a.num_blocks) {
       set_status(ERR_BAD_INDEX);
       blk = 0;             // load something valid; the result is flagged
@@ -408,29 +405,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     }
     cp_arrive_noinc((is_v ? v_full : k_full) + j % L::STAGES);
   };
-  // ---- softmax warps: the queries of the warp's 32 rows go straight to shared
-  // memory (HD/8 lanes a row; missing rows are zero) while the CTA meets
-  const int r = threadIdx.x;                       // row of a softmax thread
-  const bool valid = r < nrows;
-  const int R = rt * TT_ROWS + (valid ? r : 0);
-  const size_t row = (size_t)s.q0 + R / G;
-  unsigned long long m[TREE_WORDS] = {0, 0, 0, 0};
-  if (warp < act) {
-    constexpr int PPR = HD / 8, RPI = 32 / PPR;
-    const unsigned long long mine = row * a.ld_q + (size_t)(kvh * G + R % G) * HD;
-    const int c = lane % PPR;
-#pragma unroll
-    for (int i = 0; i < 32 / RPI; ++i) {
-      const int rr = i * RPI + lane / PPR;
-      const unsigned long long off = __shfl_sync(0xffffffffu, mine, rr);
-      cp_async16(sbase + (c >> 3) * L::Q_HALF + sw128_off(warp * 32 + rr, c & 7),
-                 a.q + off + c * 8, warp * 32 + rr < nrows);
-    }
-    cp_commit();
-#pragma unroll
-    for (int i = 0; i < TREE_WORDS; ++i)
-      if (i < t.mask_w && valid) m[i] = t.mask[row * t.mask_ld + i];
-  } else if (warp == 4 && lane == 0) {
+  if (warp == 4 && lane == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&p_full[i], 32 * act);
     mbar_init(q_full, 32 * act);
     *s_bad = 0;
@@ -441,6 +416,11 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   tc_fence_after();
   // only now: a dependent kernel that takes tensor memory must not get in before this CTA's
   if (threadIdx.x == 0) pdl_trigger();
+  const int r = threadIdx.x;                       // row of a softmax thread
+  const bool valid = r < nrows;
+  const int R = rt * TT_ROWS + (valid ? r : 0);
+  const size_t row = (size_t)s.q0 + R / G;
+  unsigned long long m[TREE_WORDS] = {0, 0, 0, 0};
   const uint32_t tmem = *tmem_slot;
   float ref = -INFINITY, l = 0.f;                  // a row's exponent reference (log2) and sum
 
@@ -449,15 +429,15 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     // their stages come free); block ids are read a window or a tile ahead
     if (TMA) {
       if (nt > 0) {
-        kid = chunks(0);
+        kid = chunks(0, rank == 0);
         issue(0, false);
       }
-      next = chunks(8);
+      next = chunks(8, false);
       for (int j = 0; j < nt; ++j) {
         vid = kid;
         if (((j + 1) & 7) == 0) {
           kid = next;
-          next = chunks(j + 9);
+          next = chunks(j + 9, false);
         }
         if (j + 1 < nt) {
           if (j + 1 >= L::STAGES &&
@@ -546,6 +526,24 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     __syncwarp();
   } else if (warp < act) {
     // ---------------- softmax: one row a thread
+    {
+      // the warp's 32 rows, HD/8 lanes a row, straight into shared memory; missing rows are zero
+      constexpr int PPR = HD / 8, RPI = 32 / PPR;
+      const unsigned long long mine = row * a.ld_q + (size_t)(kvh * G + R % G) * HD;
+      const int c = lane % PPR;
+#pragma unroll
+      for (int i = 0; i < 32 / RPI; ++i) {
+        const int rr = i * RPI + lane / PPR;
+        const unsigned long long off = __shfl_sync(0xffffffffu, mine, rr);
+        cp_async16(sbase + (c >> 3) * L::Q_HALF + sw128_off(warp * 32 + rr, c & 7),
+                   a.q + off + c * 8, warp * 32 + rr < nrows);
+      }
+      cp_commit();
+    }
+#pragma unroll
+    for (int i = 0; i < TREE_WORDS; ++i)
+      if (i < t.mask_w && valid) m[i] = t.mask[row * t.mask_ld + i];
+    s_out[r] = row * a.ld_out + (size_t)(kvh * G + R % G) * HD;
     cp_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(q_full);
@@ -641,119 +639,96 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   __syncthreads();      // every load has landed and every MMA is complete
 
   // ---------------- epilogue
-  const int j0 = max(t0 * TT_KEYS - s.base, 0);                        // this split's draft nodes
-  const int j1 = min((t0 + nt) * TT_KEYS - s.base, s.ql);
-  const bool bad = *s_bad != 0;
-  if (warp < act) {
-    const uint32_t to = tmem + L::COL_O + ((uint32_t)(warp * 32) << 16);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    __nv_bfloat16* dst =
-        a.out + row * a.ld_out + (size_t)(kvh * G + R % G) * HD;
-    float* keep = reinterpret_cast<float*>(smem) + r * L::LDO;
+  const uint32_t to = tmem + L::COL_O + ((uint32_t)((warp & 3) * 32) << 16);
+  if (C == 1) {
+    if (warp < act) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      __nv_bfloat16* dst = a.out + row * a.ld_out + (size_t)(kvh * G + R % G) * HD;
 #pragma unroll
-    for (int c0 = 0; c0 < HD; c0 += 32) {
-      float v[32];
-      if (nt > 0) {
+      for (int c0 = 0; c0 < HD; c0 += 32) {
+        float v[32];
         tmem_ld32(to + c0, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0.f;
-      }
-      if (C > 1) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 4)
-          *reinterpret_cast<float4*>(keep + c0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-      } else if (valid) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = l == 0.f ? 0.f : v[e] * inv;
+        if (valid)
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) store_bf16x8(dst + c0 + e, v + e);
+          for (int e = 0; e < 32; e += 8) store_bf16x8(dst + c0 + e, v + e);
       }
+      if (*s_bad != 0 && valid) add_nonfinite<HD>(t, table, kvh, row, s, dst);
     }
-    if (C > 1) s_ml[r] = make_float2(ref, l);
-    if (bad && valid)
-      for_nonfinite<HD>(t, table, kvh, row, s.base, j0, j1, [&](int c, float x) {
-        if (C > 1) keep[c] += x;
-        else dst[c] = __float2bfloat16_rn(__bfloat162float(dst[c]) + x);
-      });
-  }
-  tc_fence_before();
-  if (C == 1) {
+    tc_fence_before();
     __syncthreads();
   } else {
-    cluster_sync_all();
-    // this CTA's 1/C of the rows: each row's weights first, then its columns, four
-    // a lane, several remote loads in flight
-    const int per = (nrows + C - 1) / C;
-    const int r0 = min(rank * per, nrows), n = min(per, nrows - r0);
-    float* wt = reinterpret_cast<float*>(smem + L::OFF_W);
-    if (threadIdx.x < n) {
-      const int r = r0 + threadIdx.x;
+    // CTA z owns rows z * per .. of the tile: every CTA stores its O of them, and
+    // (reference, sum), into the owner's shared memory as [split][4 columns][row]
+    // (up to 512 contiguous bytes a warp instruction); the owner adds the splits up
+    // in order
+    const int per = (nrows + C - 1) / C, pitch = per | 1;
+    const bool bad = *s_bad != 0;
+    cluster_sync_all();          // every member's rings are free
+    if (warp < act) {
+      const int owner = valid ? r / per : 0, at = r - owner * per;
+      const uint32_t dst =
+          cluster_map(sbase, owner) + (uint32_t)(rank * (HD / 4) * pitch + at) * 16;
+      if (valid) st_cluster_f2(cluster_map(sbase + L::OFF_ML + (rank * per + at) * 8, owner), ref, l);
+#pragma unroll
+      for (int c0 = 0; c0 < HD; c0 += 32) {
+        float v[32];
+        if (nt > 0) {
+          tmem_ld32(to + c0, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0.f;
+        }
+        if (valid)
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            st_cluster_v4(dst + (c0 + e) / 4 * pitch * 16, v[e], v[e + 1], v[e + 2], v[e + 3]);
+      }
+    }
+    if (bad && threadIdx.x < C) st_cluster_u32(cluster_map(smem_u32(s_bad), threadIdx.x), 1u);
+    tc_fence_before();
+    cluster_sync_all();          // everything has arrived; nobody touches this CTA's memory after
+    const int r0 = rank * per, n = min(per, nrows - r0);
+    const float* so = reinterpret_cast<const float*>(smem);
+    constexpr int LPR = HD / 4;             // lanes a row, four columns each
+    constexpr int RPP = TT_THREADS / LPR;   // rows a pass
+    const int c4 = threadIdx.x % LPR;
+    const bool fix = *s_bad != 0;
+#pragma unroll 4
+    for (int i = threadIdx.x / LPR; i < n; i += RPP) {
       float2 ml[TT_MAX_SPLITS];
+      float4 o[TT_MAX_SPLITS];
       float M = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int z = 0; z < TT_MAX_SPLITS; ++z)
-        if (z < C) ml[z] = ld_cluster_f2(cluster_map(sbase + L::OFF_ML + r * 8, z));
-#pragma unroll
-      for (int z = 0; z < TT_MAX_SPLITS; ++z)
-        if (z < C) M = fmaxf(M, ml[z].x);
+        if (z < C) {
+          ml[z] = s_ml[z * per + i];
+          o[z] = *reinterpret_cast<const float4*>(so + ((z * LPR + c4) * pitch + i) * 4);
+          M = fmaxf(M, ml[z].x);
+        }
       const float mu = M == -INFINITY ? 0.f : M;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int z = 0; z < TT_MAX_SPLITS; ++z)
         if (z < C) {
-          ml[z].x = ex2_approx(ml[z].x - mu);      // 0 for a split that saw nothing
-          sum += ml[z].x * ml[z].y;
+          const float w = ex2_approx(ml[z].x - mu);     // 0 for a split that saw nothing
+          sum += w * ml[z].y;
+          acc.x += w * o[z].x, acc.y += w * o[z].y, acc.z += w * o[z].z, acc.w += w * o[z].w;
         }
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-      for (int z = 0; z < TT_MAX_SPLITS; ++z)
-        if (z < C) wt[threadIdx.x * TT_MAX_SPLITS + z] = ml[z].x * inv;
+      uint2 v;
+      v.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+      v.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(a.out + s_out[r0 + i] + c4 * 4) = v;
     }
-    __syncthreads();
-    constexpr int LPR = HD / 4, UN = 2;
-    const int items = n * LPR;
-    for (int i0 = threadIdx.x; i0 < items; i0 += UN * TT_THREADS) {
-      float4 acc[UN];
-#pragma unroll
-      for (int u = 0; u < UN; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int z0 = 0; z0 < TT_MAX_SPLITS; z0 += 4) {
-        if (z0 >= C) break;
-        float4 o[UN][4];
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          const int i = min(i0 + u * TT_THREADS, items - 1);
-          const uint32_t src = sbase + ((r0 + i / LPR) * L::LDO + (i % LPR) * 4) * 4;
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            if (z0 + z < C) o[u][z] = ld_cluster_f4(cluster_map(src, z0 + z));
-        }
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          const int i = min(i0 + u * TT_THREADS, items - 1);
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            if (z0 + z < C) {
-              const float w = wt[i / LPR * TT_MAX_SPLITS + z0 + z];
-              acc[u].x += w * o[u][z].x, acc[u].y += w * o[u][z].y;
-              acc[u].z += w * o[u][z].z, acc[u].w += w * o[u][z].w;
-            }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int i = i0 + u * TT_THREADS;
-        if (i < items) {
-          const int R = rt * TT_ROWS + r0 + i / LPR;
-          uint2 v;
-          v.x = pack_bf16x2(acc[u].x, acc[u].y);
-          v.y = pack_bf16x2(acc[u].z, acc[u].w);
-          *reinterpret_cast<uint2*>(a.out + ((size_t)s.q0 + R / G) * a.ld_out +
-                                    (size_t)(kvh * G + R % G) * HD + (i % LPR) * 4) = v;
-        }
+    if (fix) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += TT_THREADS) {
+        const int Ri = rt * TT_ROWS + r0 + i;
+        add_nonfinite<HD>(t, table, kvh, (size_t)s.q0 + Ri / G, s, a.out + s_out[r0 + i]);
       }
     }
-    cluster_sync_all();   // peers read this CTA's shared memory until here
   }
   if (warp == 5) {
     tc_fence_after();
