@@ -22,6 +22,7 @@ struct TreeAttnArgs {
   int mask_ld, mask_w;
   int n_rows;                             // rows of q, out and mask
   int max_q;                              // the grid covers max_q nodes a sequence
+  bool by_length;                         // blockIdx.z-th longest sequence instead of number blockIdx.z
   int bt_w;                               // columns of a block-table row (a.bt_ld: its pitch)
 };
 
@@ -182,28 +183,47 @@ constexpr int TT_THREADS = 192;
 constexpr float TT_RESCALE = 8.f;
 constexpr int TT_MAX_SPLITS = 8;
 
+// Shared memory of a CTA: Q (only the warps' rows that exist: the MMA reads 128
+// rows whatever they hold, the others' results are never looked at), then as many
+// stages of K and of V as fit half an SM.
 template <int HD>
 struct TreeTcLayout {
   static constexpr int HALVES = HD / 64;
-  static constexpr int Q_HALF = TT_ROWS * 128;
-  static constexpr int Q_TILE = HALVES * Q_HALF;
   static constexpr int GROUP = HALVES * 1024;          // 8 tokens of K (or V)
   static constexpr int BOX = 2 * GROUP;                // 16 tokens
   static constexpr int STAGE = TT_KEYS / 8 * GROUP;
-  static constexpr int STAGES = HD == 128 ? 2 : 4;     // of K and of V
-  static constexpr int OFF_K = Q_TILE;
-  static constexpr int OFF_V = OFF_K + STAGES * STAGE;
-  static constexpr int OFF_ML = OFF_V + STAGES * STAGE;
-  static constexpr int OFF_OUT = OFF_ML + (TT_ROWS + TT_MAX_SPLITS) * 8;   // rows' places in out
-  static constexpr int OFF_BAR = OFF_OUT + TT_ROWS * 8;
-  static constexpr int N_BARS = 4 * STAGES + 7;
-  static constexpr int SMEM = OFF_BAR + 32 * 8 + 1024;
+  static constexpr int MAX_STAGES = HD == 128 ? 3 : 6; // of K, of V
+  static constexpr int DATA = 112 * 1024;              // Q and the rings; then the merge:
+  static constexpr int OFF_ML = DATA - 4096;           // (reference, sum) of the splits' rows
+  static constexpr int OFF_OUT = DATA - 2048;          // rows' places in out
+  static constexpr int OFF_BAR = DATA;
+  static constexpr int N_BARS = 4 * MAX_STAGES + 7;
+  static constexpr int SMEM = OFF_BAR + 512 + 512;     // barriers; alignment slack
   static constexpr uint32_t COL_O = 2 * TT_KEYS;
   static constexpr uint32_t TMEM_COLS = 256;
+  __device__ static constexpr int q_half(int act) { return act * 4096; }   // 32 rows a warp
+  __device__ static constexpr int stages(int act) { return (DATA - HALVES * q_half(act)) / STAGE; }
+  __device__ static constexpr int v_stages(int act) {
+    return stages(act) / 2 < MAX_STAGES ? stages(act) / 2 : MAX_STAGES;
+  }
+  __device__ static constexpr int k_stages(int act) {
+    return stages(act) - v_stages(act) < MAX_STAGES ? stages(act) - v_stages(act) : MAX_STAGES;
+  }
   static_assert((TT_ROWS + 2 * TT_MAX_SPLITS) * HD * 4 <= OFF_ML, "merged rows over Q and the rings");
-  static_assert(N_BARS * 8 + 8 <= 32 * 8, "barrier area");
+  static_assert((TT_ROWS + TT_MAX_SPLITS) * 8 <= OFF_OUT - OFF_ML && TT_ROWS * 8 <= DATA - OFF_OUT,
+                "merge tables");
+  static_assert(N_BARS * 8 + 12 <= 512, "barrier area");
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
   static_assert(2 * TT_KEYS + HD <= 256, "TMEM: two S buffers and O in half of it");
+};
+
+// Position in a ring of n stages; `phase` flips with every lap.
+struct RingPos {
+  int st = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++st == n) st = 0, phase ^= 1;
+  }
 };
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar,
@@ -290,21 +310,26 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   uint8_t* smem = align_smem_1024(smem_raw);
   float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
   size_t* s_out = reinterpret_cast<size_t*>(smem + L::OFF_OUT);
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR); // [STAGES]
-  uint64_t* k_empty = k_full + L::STAGES;                           // [STAGES]
-  uint64_t* v_full = k_empty + L::STAGES;                           // [STAGES]
-  uint64_t* v_empty = v_full + L::STAGES;                           // [STAGES]
-  uint64_t* s_full = v_empty + L::STAGES;                           // [2]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* k_empty = k_full + L::MAX_STAGES;
+  uint64_t* v_full = k_empty + L::MAX_STAGES;
+  uint64_t* v_empty = v_full + L::MAX_STAGES;
+  uint64_t* s_full = v_empty + L::MAX_STAGES;                       // [2]
   uint64_t* p_full = s_full + 2;                                    // [2]
   uint64_t* pv_done = p_full + 2;                                   // [2]
   uint64_t* q_full = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   int* s_bad = reinterpret_cast<int*>(tmem_slot + 1);   // a draft's V has non-finite elements
+  int* s_seq = s_bad + 1;
 
+  if (smem - smem_raw > 512) {   // (dynamic shared memory starts 1 KiB aligned)
+    pdl_wait();
+    set_status(ERR_BAD_INDEX);
+    return;
+  }
   const AttnArgs& a = t.a;
   const int C = gridDim.x, rank = blockIdx.x;     // cluster = (C, 1, 1)
   const int kvh = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles;
-  const int seq = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t sbase = smem_u32(smem);
   if (warp == 5) {
@@ -312,7 +337,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     tmem_relinquish();
   } else if (warp == 4) {
     if (lane == 0) {
-      for (int i = 0; i < L::STAGES; ++i) {
+      for (int i = 0; i < L::MAX_STAGES; ++i) {
         mbar_init(&k_full[i], TMA ? 1 : 32);
         mbar_init(&k_empty[i], 1);
         mbar_init(&v_full[i], TMA ? 1 : 32);
@@ -328,6 +353,23 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     __syncwarp();
   }
   pdl_wait();
+  int seq = blockIdx.z;
+  if (t.by_length) {       // (at most 64 sequences) this one is the blockIdx.z-th longest
+    if (warp == 5) {
+      const int n = a.n_seqs;
+      const int c0 = lane < n ? a.ctx_len[lane] : 0, c1 = lane + 32 < n ? a.ctx_len[lane + 32] : 0;
+      int k0 = 0, k1 = 0;
+      for (int j = 0; j < n; ++j) {
+        const int v = __shfl_sync(0xffffffffu, j < 32 ? c0 : c1, j & 31);
+        k0 += v > c0 || (v == c0 && j < lane);
+        k1 += v > c1 || (v == c1 && j < lane + 32);
+      }
+      if (lane < n && k0 == seq) *s_seq = lane;
+      if (lane + 32 < n && k1 == seq) *s_seq = lane + 32;
+    }
+    __syncthreads();
+    seq = *s_seq;
+  }
   const int* table = a.block_tables + (size_t)seq * a.bt_ld;
   // the first split starts at token 0: its block ids need not wait for the metadata
   int early = 0;
@@ -348,6 +390,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   const unsigned tiles = (unsigned)(s.ctx + TT_KEYS - 1) / TT_KEYS;   // (below 2^26: times C fits)
   const int t0 = (int)(tiles * rank / C);
   const int nt = (int)(tiles * (rank + 1) / C) - t0;
+  const int q_half = L::q_half(act), KS = L::k_stages(act), VS = L::v_stages(act);
+  const int off_k = L::HALVES * q_half, off_v = off_k + KS * L::STAGE;
 
   // ---- loader state (warp 4)
   // TMA: lane i holds the 8-token group of K of chunk i (16 tokens) of eight tiles
@@ -363,15 +407,14 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     return (blk * 2 * a.n_kv_heads + kvh) * (a.block_size / 8) + c * 16 % a.block_size / 8;
   };
   const int v_off = a.n_kv_heads * (a.block_size / 8);   // from K's group to V's
-  auto issue = [&](int j, bool is_v) {
-    const int st = j & (L::STAGES - 1);
+  auto issue = [&](int j, bool is_v, int st) {
     const int g = __shfl_sync(0xffffffffu, is_v ? vid : kid, ((j & 7) * 4 + lane) & 31);
     const int left = (s.ctx - (t0 + j) * TT_KEYS + 15) / 16;   // boxes of the tile
     uint64_t* full = (is_v ? v_full : k_full) + st;
     if (lane == 0) mbar_arrive_expect_tx(full, min(left, TT_KEYS / 16) * L::BOX);
     __syncwarp();
     if (lane < min(left, TT_KEYS / 16))
-      tma_load_4d(smem + (is_v ? L::OFF_V : L::OFF_K) + st * L::STAGE + lane * L::BOX, &map, full,
+      tma_load_4d(smem + (is_v ? off_v : off_k) + st * L::STAGE + lane * L::BOX, &map, full,
                   is_v ? g + v_off : g);
   };
   // cp.async: pool rows (of hd elements) of keys lane and lane + 32 of a tile
@@ -390,9 +433,9 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       }
     }
   };
-  auto copy = [&](int j, const unsigned* row, bool is_v) {
+  auto copy = [&](const unsigned* row, bool is_v, int at) {
     constexpr int PPR = HD / 8, RPI = 32 / PPR;    // lanes a row, rows an instruction
-    const uint32_t st = sbase + (is_v ? L::OFF_V : L::OFF_K) + (j % L::STAGES) * L::STAGE;
+    const uint32_t st = sbase + (is_v ? off_v : off_k) + at * L::STAGE;
     const int c = lane % PPR;
     const __nv_bfloat16* src =
         a.pool + c * 8 + (is_v ? (size_t)a.n_kv_heads * a.block_size * HD : 0);
@@ -403,7 +446,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       cp_async16(st + (key >> 3) * L::GROUP + (c >> 3) * 1024 + sw128_off(key & 7, c & 7),
                  src + (r != ~0u ? (size_t)r * HD : 0), r != ~0u);
     }
-    cp_arrive_noinc((is_v ? v_full : k_full) + j % L::STAGES);
+    cp_arrive_noinc((is_v ? v_full : k_full) + at);
   };
   if (warp == 4 && lane == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&p_full[i], 32 * act);
@@ -427,10 +470,15 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   if (warp == 4) {
     // ---------------- loader: K of tile j + 1, then V of tile j (the order in which
     // their stages come free); block ids are read a window or a tile ahead
+    RingPos kp, vp;
+    auto room = [&](uint64_t* empty, const RingPos& p) {   // the stage's last user is done
+      return __all_sync(0xffffffffu, mbar_wait(&empty[p.st], p.phase ^ 1)) != 0;
+    };
     if (TMA) {
       if (nt > 0) {
         kid = chunks(0, rank == 0);
-        issue(0, false);
+        issue(0, false, 0);
+        kp.next(KS);
       }
       next = chunks(8, false);
       for (int j = 0; j < nt; ++j) {
@@ -440,22 +488,19 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
           next = chunks(j + 9, false);
         }
         if (j + 1 < nt) {
-          if (j + 1 >= L::STAGES &&
-              !__all_sync(0xffffffffu, mbar_wait(&k_empty[(j + 1) & (L::STAGES - 1)],
-                                                 ((j + 1) / L::STAGES - 1) & 1)))
-            break;
-          issue(j + 1, false);
+          if (!room(k_empty, kp)) break;
+          issue(j + 1, false, kp.st);
+          kp.next(KS);
         }
-        if (j >= L::STAGES &&
-            !__all_sync(0xffffffffu, mbar_wait(&v_empty[j & (L::STAGES - 1)],
-                                               (j / L::STAGES - 1) & 1)))
-          break;
-        issue(j, true);
+        if (!room(v_empty, vp)) break;
+        issue(j, true, vp.st);
+        vp.next(VS);
       }
     } else {
       if (nt > 0) {
         find(0, krow);
-        copy(0, krow, false);
+        copy(krow, false, 0);
+        kp.next(KS);
       }
       if (nt > 1) find(1, nrow);
       for (int j = 0; j < nt; ++j) {
@@ -463,16 +508,13 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
         if (j + 1 < nt) {
           krow[0] = nrow[0], krow[1] = nrow[1];
           if (j + 2 < nt) find(j + 2, nrow);
-          if (j + 1 >= L::STAGES &&
-              !__all_sync(0xffffffffu, mbar_wait(&k_empty[(j + 1) % L::STAGES],
-                                                 ((j + 1) / L::STAGES - 1) & 1)))
-            break;
-          copy(j + 1, krow, false);
+          if (!room(k_empty, kp)) break;
+          copy(krow, false, kp.st);
+          kp.next(KS);
         }
-        if (j >= L::STAGES &&
-            !__all_sync(0xffffffffu, mbar_wait(&v_empty[j % L::STAGES], (j / L::STAGES - 1) & 1)))
-          break;
-        copy(j, vrow, true);
+        if (!room(v_empty, vp)) break;
+        copy(vrow, true, vp.st);
+        vp.next(VS);
       }
       cp_wait<0>();   // nothing in flight at exit
     }
@@ -481,25 +523,25 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     if (lane == 0 && nt > 0) {
       constexpr uint32_t idesc_s = idesc_bf16_m128(TT_KEYS);
       constexpr uint32_t idesc_o = idesc_bf16_m128(HD) | (1u << 16);   // V: MN-major
+      RingPos kp, vp;
       auto issue_s = [&](int j) -> bool {
-        const int st = j % L::STAGES;
-        if (!mbar_wait(&k_full[st], (j / L::STAGES) & 1)) return false;
+        if (!mbar_wait(&k_full[kp.st], kp.phase)) return false;
         tc_fence_after();
         if (!TMA) fence_proxy_async_smem();   // K arrived through the generic proxy
-        const uint32_t kb = sbase + L::OFF_K + st * L::STAGE;
+        const uint32_t kb = sbase + off_k + kp.st * L::STAGE;
 #pragma unroll
         for (int h = 0; h < L::HALVES; ++h)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            tc_mma_bf16(tmem + (j & 1) * TT_KEYS, sw128_desc(sbase + h * L::Q_HALF + kk * 32),
+            tc_mma_bf16(tmem + (j & 1) * TT_KEYS, sw128_desc(sbase + h * q_half + kk * 32),
                         sw128_k_desc(kb + h * 1024 + kk * 32, L::GROUP), idesc_s,
                         (h | kk) ? 1u : 0u);
         tc_commit(&s_full[j & 1]);
-        tc_commit(&k_empty[st]);
+        tc_commit(&k_empty[kp.st]);
+        kp.next(KS);
         return true;
       };
       bool good = mbar_wait(q_full, 0);
-      tc_fence_after();
       if (good) good = issue_s(0);
       for (int j = 0; j < nt && good; ++j) {
         if (j + 1 < nt) {
@@ -508,19 +550,19 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
           if (good) good = issue_s(j + 1);
           if (!good) break;
         }
-        const int st = j % L::STAGES;
-        if (!mbar_wait(&v_full[st], (j / L::STAGES) & 1)) break;
+        if (!mbar_wait(&v_full[vp.st], vp.phase)) break;
         if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1)) break;
         tc_fence_after();
         if (!TMA) fence_proxy_async_smem();   // V too
-        const uint32_t vb = sbase + L::OFF_V + st * L::STAGE;
+        const uint32_t vb = sbase + off_v + vp.st * L::STAGE;
 #pragma unroll
         for (int ks = 0; ks < TT_KEYS / 16; ++ks)
           tc_mma_bf16_ts(tmem + L::COL_O, tmem + (j & 1) * TT_KEYS + ks * 8,
                          sw128_mn_desc(vb + ks * 2 * L::GROUP, 1024, L::GROUP), idesc_o,
                          (j | ks) ? 1u : 0u);
-        tc_commit(&v_empty[st]);
+        tc_commit(&v_empty[vp.st]);
         tc_commit(&pv_done[j & 1]);
+        vp.next(VS);
       }
     }
     __syncwarp();
@@ -535,7 +577,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       for (int i = 0; i < 32 / RPI; ++i) {
         const int rr = i * RPI + lane / PPR;
         const unsigned long long off = __shfl_sync(0xffffffffu, mine, rr);
-        cp_async16(sbase + (c >> 3) * L::Q_HALF + sw128_off(warp * 32 + rr, c & 7),
+        cp_async16(sbase + (c >> 3) * q_half + sw128_off(warp * 32 + rr, c & 7),
                    a.q + off + c * 8, warp * 32 + rr < nrows);
       }
       cp_commit();
@@ -543,7 +585,6 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
 #pragma unroll
     for (int i = 0; i < TREE_WORDS; ++i)
       if (i < t.mask_w && valid) m[i] = t.mask[row * t.mask_ld + i];
-    s_out[r] = row * a.ld_out + (size_t)(kvh * G + R % G) * HD;
     cp_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(q_full);
@@ -566,9 +607,9 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
           if (!(wl & (1u << e))) x[e] = -INFINITY;
           if (!(wh & (1u << e))) x[32 + e] = -INFINITY;
         }
-        const int st = j % L::STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / L::STAGES) & 1))) break;
-        uint8_t* vb = smem + L::OFF_V + st * L::STAGE;
+        const int lap = j / VS, st = j - lap * VS;
+        if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], lap & 1))) break;
+        uint8_t* vb = smem + off_v + st * L::STAGE;
         const int first = max(s.base - k0, 0);
         for (int i = first * (HD / 8) + r; i < TT_KEYS * (HD / 8); i += 32 * act) {
           const int key = i / (HD / 8), c = i % (HD / 8);
@@ -665,6 +706,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     // in order
     const int per = (nrows + C - 1) / C, pitch = per | 1;
     const bool bad = *s_bad != 0;
+    if (warp < act) s_out[r] = row * a.ld_out + (size_t)(kvh * G + R % G) * HD;
     cluster_sync_all();          // every member's rings are free
     if (warp < act) {
       const int owner = valid ? r / per : 0, at = r - owner * per;
@@ -773,7 +815,7 @@ static int tree_splits(int n_seqs, int n_kv, int row_tiles, int max_ctx, long lo
 }
 
 template <int HD, bool TMA>
-static int tree_tc_launch(const TreeAttnArgs& t, int max_ctx, long long ctx_total, cudaStream_t st) {
+static int tree_tc_launch(TreeAttnArgs t, int max_ctx, long long ctx_total, cudaStream_t st) {
   using L = TreeTcLayout<HD>;
   static std::atomic<unsigned long long> attr_devs{0};
   if (int rc = smem_attr_once(tree_attn_tc_kernel<HD, TMA>, L::SMEM, attr_devs,
@@ -786,6 +828,11 @@ static int tree_tc_launch(const TreeAttnArgs& t, int max_ctx, long long ctx_tota
   const int row_tiles = (int)((rows + TT_ROWS - 1) / TT_ROWS);
   if ((long long)row_tiles * t.a.n_kv_heads > 65535) return arg_err("too many heads and nodes");
   const int C = tree_splits(t.a.n_seqs, t.a.n_kv_heads, row_tiles, max_ctx, ctx_total);
+  // More CTAs than fit at once and ragged, long contexts: longest sequences first,
+  // so that none starts late (ranking them costs ~0.5 us a CTA)
+  const int n = t.a.n_seqs;
+  t.by_length = n > 1 && n <= 64 && (long long)C * t.a.n_kv_heads * row_tiles * n > 148 * 2 &&
+                4ll * max_ctx * n > 5 * ctx_total && max_ctx / C >= 1024;
   return launch_pdl(tree_attn_tc_kernel<HD, TMA>, dim3(C, t.a.n_kv_heads * row_tiles, t.a.n_seqs),
                     dim3(TT_THREADS), L::SMEM, st, C, "tree attention launch", map, t, row_tiles);
 }
