@@ -23,6 +23,9 @@ struct TreeAttnArgs {
   int n_rows;                             // rows of q, out and mask
   int max_q;                              // the grid covers max_q nodes a sequence
   bool by_length;                         // blockIdx.z-th longest sequence instead of number blockIdx.z
+  int group;                              // G = n_q_heads / n_kv_heads
+  unsigned group_magic;                   // ceil(2^32 / G): r / G = umulhi(r, magic) for r < 2^16, G > 1
+  int log_splits;                         // log2 C
   int bt_w;                               // columns of a block-table row (a.bt_ld: its pitch)
 };
 
@@ -31,6 +34,9 @@ struct TreeAttnArgs {
 struct TreeSeq {
   int q0, ql, ctx, base;
 };
+__device__ __forceinline__ int div_group(const TreeAttnArgs& t, int r) {
+  return t.group == 1 ? r : (int)__umulhi((unsigned)r, t.group_magic);
+}
 __device__ __forceinline__ bool tree_seq(const TreeAttnArgs& t, int seq, TreeSeq& s) {
   s.q0 = t.a.q_start[seq];
   s.ql = t.a.q_len[seq];
@@ -38,7 +44,7 @@ __device__ __forceinline__ bool tree_seq(const TreeAttnArgs& t, int seq, TreeSeq
   s.base = s.ctx - s.ql;
   return s.ql >= 0 && s.ql <= t.max_q && s.ql <= 64 * t.mask_w && s.base >= 0 && s.q0 >= 0 &&
          s.q0 <= t.n_rows - s.ql &&
-         (int)(((long long)s.ctx + t.a.block_size - 1) / t.a.block_size) <= t.bt_w;
+         s.ctx <= (long long)t.bt_w * t.a.block_size;
 }
 
 // ------------------------------------------------------------ short heads
@@ -301,6 +307,49 @@ __device__ __forceinline__ void add_nonfinite(const TreeAttnArgs& t, const int* 
   }
 }
 
+// Every thread of a cluster arrives and waits; nothing is published.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile(
+      "barrier.cluster.arrive.relaxed.aligned;\n\t"
+      "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The rows a CTA owns: out = sum_z w_z O_z / sum_z w_z l_z, w_z = 2^(ref_z - max ref).
+template <int HD, int C>
+__device__ __forceinline__ void merge_rows(const uint8_t* smem, const float2* s_ml,
+                                           const size_t* s_out, __nv_bfloat16* out, int per,
+                                           int pitch, int n) {
+  constexpr int LPR = HD / 4;             // lanes a row, four columns each
+  constexpr int RPP = TT_THREADS / LPR;   // rows a pass
+  const float* so = reinterpret_cast<const float*>(smem);
+  const int c4 = threadIdx.x % LPR;
+#pragma unroll (8 / C)
+  for (int i = threadIdx.x / LPR; i < n; i += RPP) {
+    float2 ml[C];
+    float4 o[C];
+    float M = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int z = 0; z < C; ++z) {
+      ml[z] = s_ml[z * per + i];
+      o[z] = *reinterpret_cast<const float4*>(so + ((z * LPR + c4) * pitch + i) * 4);
+      M = fmaxf(M, ml[z].x);
+    }
+    const float mu = M == -INFINITY ? 0.f : M;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int z = 0; z < C; ++z) {
+      const float w = ex2_approx(ml[z].x - mu);   // 0 for a split that saw nothing
+      sum += w * ml[z].y;
+      acc.x += w * o[z].x, acc.y += w * o[z].y, acc.z += w * o[z].z, acc.w += w * o[z].w;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint2 v;
+    v.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+    v.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(out + s_out[i] + c4 * 4) = v;
+  }
+}
+
 template <int HD, bool TMA>
 __global__ void __launch_bounds__(TT_THREADS, 2)
     tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map, const TreeAttnArgs t,
@@ -336,20 +385,15 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     tmem_alloc(tmem_slot, L::TMEM_COLS);
     tmem_relinquish();
   } else if (warp == 4) {
-    if (lane == 0) {
-      for (int i = 0; i < L::MAX_STAGES; ++i) {
-        mbar_init(&k_full[i], TMA ? 1 : 32);
-        mbar_init(&k_empty[i], 1);
-        mbar_init(&v_full[i], TMA ? 1 : 32);
-        mbar_init(&v_empty[i], 1);
-      }
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&s_full[i], 1);
-        mbar_init(&pv_done[i], 1);
-      }
-      fence_mbar_init();
-      if (TMA) prefetch_tmap(&map);
+    // full and empty barriers of K, then of V, then the S and P V ones
+    if (lane < 4 * L::MAX_STAGES)
+      mbar_init(&k_full[lane], !TMA && (lane / L::MAX_STAGES) % 2 == 0 ? 32 : 1);
+    if (lane < 2) {
+      mbar_init(&s_full[lane], 1);
+      mbar_init(&pv_done[lane], 1);
     }
+    fence_mbar_init();
+    if (TMA && lane == 0) prefetch_tmap(&map);
     __syncwarp();
   }
   pdl_wait();
@@ -377,7 +421,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     early = table[lane * 16 / a.block_size];
   TreeSeq s;
   const bool ok = tree_seq(t, seq, s);
-  const int G = a.n_q_heads / a.n_kv_heads;
+  const int G = t.group;
   const int rows = s.ql * G - rt * TT_ROWS;        // of this tile on
   if (!ok || rows <= 0) {                          // uniform over the cluster
     if (!ok && rt == 0 && threadIdx.x == 0) set_status(ERR_BAD_INDEX);
@@ -388,8 +432,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   const int nrows = min(rows, TT_ROWS);
   const int act = (nrows + 31) / 32;               // softmax warps with rows
   const unsigned tiles = (unsigned)(s.ctx + TT_KEYS - 1) / TT_KEYS;   // (below 2^26: times C fits)
-  const int t0 = (int)(tiles * rank / C);
-  const int nt = (int)(tiles * (rank + 1) / C) - t0;
+  const int t0 = (int)(tiles * rank >> t.log_splits);
+  const int nt = (int)(tiles * (rank + 1) >> t.log_splits) - t0;
   const int q_half = L::q_half(act), KS = L::k_stages(act), VS = L::v_stages(act);
   const int off_k = L::HALVES * q_half, off_v = off_k + KS * L::STAGE;
 
@@ -461,8 +505,9 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   if (threadIdx.x == 0) pdl_trigger();
   const int r = threadIdx.x;                       // row of a softmax thread
   const bool valid = r < nrows;
-  const int R = rt * TT_ROWS + (valid ? r : 0);
-  const size_t row = (size_t)s.q0 + R / G;
+  const int R = rt * TT_ROWS + (valid ? r : 0), node = div_group(t, R);
+  const size_t row = (size_t)s.q0 + node;
+  const int col = (kvh * G + R - node * G) * HD;   // the row's place in q and out
   unsigned long long m[TREE_WORDS] = {0, 0, 0, 0};
   const uint32_t tmem = *tmem_slot;
   float ref = -INFINITY, l = 0.f;                  // a row's exponent reference (log2) and sum
@@ -571,7 +616,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     {
       // the warp's 32 rows, HD/8 lanes a row, straight into shared memory; missing rows are zero
       constexpr int PPR = HD / 8, RPI = 32 / PPR;
-      const unsigned long long mine = row * a.ld_q + (size_t)(kvh * G + R % G) * HD;
+      const unsigned long long mine = row * a.ld_q + col;
       const int c = lane % PPR;
 #pragma unroll
       for (int i = 0; i < 32 / RPI; ++i) {
@@ -677,14 +722,16 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       tc_fence_after();
     }
   }
-  __syncthreads();      // every load has landed and every MMA is complete
 
-  // ---------------- epilogue
+  // ---------------- epilogue.  Past the barrier every load of the CTA (with C > 1: of
+  // every member) has landed and every MMA is complete
+  if (C == 1) __syncthreads();
+  else cluster_sync_relaxed();
   const uint32_t to = tmem + L::COL_O + ((uint32_t)((warp & 3) * 32) << 16);
   if (C == 1) {
     if (warp < act) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      __nv_bfloat16* dst = a.out + row * a.ld_out + (size_t)(kvh * G + R % G) * HD;
+      __nv_bfloat16* dst = a.out + row * a.ld_out + col;
 #pragma unroll
       for (int c0 = 0; c0 < HD; c0 += 32) {
         float v[32];
@@ -705,10 +752,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     // (up to 512 contiguous bytes a warp instruction); the owner adds the splits up
     // in order
     const int per = (nrows + C - 1) / C, pitch = per | 1;
-    const bool bad = *s_bad != 0;
-    if (warp < act) s_out[r] = row * a.ld_out + (size_t)(kvh * G + R % G) * HD;
-    cluster_sync_all();          // every member's rings are free
     if (warp < act) {
+      s_out[r] = row * a.ld_out + col;
       const int owner = valid ? r / per : 0, at = r - owner * per;
       const uint32_t dst =
           cluster_map(sbase, owner) + (uint32_t)(rank * (HD / 4) * pitch + at) * 16;
@@ -728,47 +773,20 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
             st_cluster_v4(dst + (c0 + e) / 4 * pitch * 16, v[e], v[e + 1], v[e + 2], v[e + 3]);
       }
     }
-    if (bad && threadIdx.x < C) st_cluster_u32(cluster_map(smem_u32(s_bad), threadIdx.x), 1u);
+    if (*s_bad != 0 && threadIdx.x < C)
+      st_cluster_u32(cluster_map(smem_u32(s_bad), threadIdx.x), 1u);
     tc_fence_before();
     cluster_sync_all();          // everything has arrived; nobody touches this CTA's memory after
     const int r0 = rank * per, n = min(per, nrows - r0);
-    const float* so = reinterpret_cast<const float*>(smem);
-    constexpr int LPR = HD / 4;             // lanes a row, four columns each
-    constexpr int RPP = TT_THREADS / LPR;   // rows a pass
-    const int c4 = threadIdx.x % LPR;
     const bool fix = *s_bad != 0;
-#pragma unroll 4
-    for (int i = threadIdx.x / LPR; i < n; i += RPP) {
-      float2 ml[TT_MAX_SPLITS];
-      float4 o[TT_MAX_SPLITS];
-      float M = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int z = 0; z < TT_MAX_SPLITS; ++z)
-        if (z < C) {
-          ml[z] = s_ml[z * per + i];
-          o[z] = *reinterpret_cast<const float4*>(so + ((z * LPR + c4) * pitch + i) * 4);
-          M = fmaxf(M, ml[z].x);
-        }
-      const float mu = M == -INFINITY ? 0.f : M;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int z = 0; z < TT_MAX_SPLITS; ++z)
-        if (z < C) {
-          const float w = ex2_approx(ml[z].x - mu);     // 0 for a split that saw nothing
-          sum += w * ml[z].y;
-          acc.x += w * o[z].x, acc.y += w * o[z].y, acc.z += w * o[z].z, acc.w += w * o[z].w;
-        }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      uint2 v;
-      v.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-      v.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(a.out + s_out[r0 + i] + c4 * 4) = v;
-    }
+    if (C == 2) merge_rows<HD, 2>(smem, s_ml, s_out + r0, a.out, per, pitch, n);
+    else if (C == 4) merge_rows<HD, 4>(smem, s_ml, s_out + r0, a.out, per, pitch, n);
+    else merge_rows<HD, 8>(smem, s_ml, s_out + r0, a.out, per, pitch, n);
     if (fix) {
       __syncthreads();
       for (int i = threadIdx.x; i < n; i += TT_THREADS) {
         const int Ri = rt * TT_ROWS + r0 + i;
-        add_nonfinite<HD>(t, table, kvh, (size_t)s.q0 + Ri / G, s, a.out + s_out[r0 + i]);
+        add_nonfinite<HD>(t, table, kvh, (size_t)s.q0 + div_group(t, Ri), s, a.out + s_out[r0 + i]);
       }
     }
   }
@@ -828,6 +846,7 @@ static int tree_tc_launch(TreeAttnArgs t, int max_ctx, long long ctx_total, cuda
   const int row_tiles = (int)((rows + TT_ROWS - 1) / TT_ROWS);
   if ((long long)row_tiles * t.a.n_kv_heads > 65535) return arg_err("too many heads and nodes");
   const int C = tree_splits(t.a.n_seqs, t.a.n_kv_heads, row_tiles, max_ctx, ctx_total);
+  t.log_splits = C == 8 ? 3 : C == 4 ? 2 : C - 1;
   // More CTAs than fit at once and ragged, long contexts: longest sequences first,
   // so that none starts late (ranking them costs ~0.5 us a CTA)
   const int n = t.a.n_seqs;
@@ -862,6 +881,8 @@ int tree_attention(TreeAttnArgs t, int head_dim, int max_ctx, long long ctx_tota
   for (const void* p : {(const void*)a.q, (const void*)a.out, (const void*)a.pool})
     if (reinterpret_cast<uintptr_t>(p) % 16) return arg_err("q / out / kv_pool must be 16-byte aligned");
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
+  t.group = a.n_q_heads / a.n_kv_heads;
+  t.group_magic = (unsigned)((0x100000000ull + t.group - 1) / t.group);
   const long long width = (long long)t.bt_w * a.block_size;   // tokens a table row can hold
   if (max_ctx <= 0 || max_ctx > width) max_ctx = (int)(width < 0x7fffffff ? width : 0x7fffffff);
   if (ctx_total <= 0 || ctx_total > (long long)max_ctx * a.n_seqs)
