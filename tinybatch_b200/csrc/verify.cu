@@ -36,6 +36,7 @@ constexpr int VF_NODES = 256;      // nodes of a sequence's tree
 constexpr int VF_MAX_WARPS = 16;
 constexpr int VF_MAX_CLUSTER = 16;
 constexpr int VF_BATCHES = 32;     // sums a warp keeps of its part of the vocabulary
+constexpr int VF_PER_LANE = VF_MAX_CLUSTER * VF_MAX_WARPS / 32;   // segments a lane looks at
 
 struct TreeArgs {
   const int *ids, *parents, *q_start, *q_len;
@@ -154,22 +155,22 @@ __device__ __forceinline__ float4 load4(const float* row, int y, int end, bool v
                      y + 2 < end ? __ldg(row + y + 2) : 0.f, y + 3 < end ? __ldg(row + y + 3) : 0.f);
 }
 
-// r of tokens y + 128 g .. + 3, g < GROUPS (y already the lane's; 0 from
-// `end` on).  All loads are issued before the first is used.
-template <bool DIST, int GROUPS>
-__device__ __forceinline__ void weights(const Rejections& h, const float* p, const float* d, int y,
-                                        int end, bool vec, double (*w)[4]) {
+// r of tokens y + STRIDE g .. + 3, g < GROUPS (y already the lane's, base the
+// warp's; 0 from `end` on).  All loads are issued before the first is used.
+template <bool DIST, int GROUPS, int STRIDE>
+__device__ __forceinline__ void weights(const Rejections& h, const float* p, const float* d,
+                                        int base, int y, int end, bool vec, double (*w)[4]) {
   float4 pv[GROUPS], dv[GROUPS];
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) pv[g] = load4(p, y + 128 * g, end, vec);
+  for (int g = 0; g < GROUPS; ++g) pv[g] = load4(p, y + STRIDE * g, end, vec);
   if (DIST)
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) dv[g] = load4(d, y + 128 * g, end, vec);
+    for (int g = 0; g < GROUPS; ++g) dv[g] = load4(d, y + STRIDE * g, end, vec);
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g)
     w[g][0] = pv[g].x, w[g][1] = pv[g].y, w[g][2] = pv[g].z, w[g][3] = pv[g].w;
   // the warp's stretch holds a rejected token (rare): only then are tokens compared
-  const bool special = rejected(h, y & ~127, 128 * GROUPS);
+  const bool special = rejected(h, base, 128 * GROUPS);
   for (int k = 0; k < h.n; ++k) {
     if (DIST) {
       const double sc = h.scale[k], iz = h.inv_z[k];
@@ -193,18 +194,54 @@ __device__ __forceinline__ void weights(const Rejections& h, const float* p, con
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         if (DIST) {
-          if (x == 128 * g) dv[g].x = 0.f;
-          if (x == 128 * g + 1) dv[g].y = 0.f;
-          if (x == 128 * g + 2) dv[g].z = 0.f;
-          if (x == 128 * g + 3) dv[g].w = 0.f;
+          if (x == STRIDE * g) dv[g].x = 0.f;
+          if (x == STRIDE * g + 1) dv[g].y = 0.f;
+          if (x == STRIDE * g + 2) dv[g].z = 0.f;
+          if (x == STRIDE * g + 3) dv[g].w = 0.f;
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (x == 128 * g + e) w[g][e] = 0.0;
+            if (x == STRIDE * g + e) w[g][e] = 0.0;
         }
       }
     }
   }
+}
+
+// Where in the sequence of all lanes' N values (lane after lane) the running sum
+// passes a target: the last positive value whose exclusive prefix does not exceed
+// it.  Some value qualifies whenever one is positive, and every warp that asks about
+// the same values picks the same one, however the prefixes are rounded.  at: the
+// target, with `fraction` as a fraction of the sum; afterwards relative to the value.
+// total: the sum.  -1: nothing is positive.
+template <int N>
+__device__ __forceinline__ int locate(const double* v, bool fraction, double& at, double& total) {
+  const int lane = threadIdx.x & 31;
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) sum += v[k];
+  double inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  total = __shfl_sync(0xffffffffu, inc, 31);
+  if (fraction) at = fmax(at * total, 0.0);   // a NaN aims at 0
+  double ex = __shfl_up_sync(0xffffffffu, inc, 1);
+  if (lane == 0) ex = 0.0;
+  const unsigned some = __ballot_sync(0xffffffffu, sum > 0.0 && ex <= at);
+  if (some == 0) return -1;
+  const int from = 31 - __clz(some);
+  int mine = 0;
+  double run = ex, before = ex;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (v[k] > 0.0 && run <= at) mine = k, before = run;
+    run += v[k];
+  }
+  at -= __shfl_sync(0xffffffffu, before, from);
+  return from * N + __shfl_sync(0xffffffffu, mine, from);
 }
 
 // One cluster a sequence, the vocabulary cut into one segment a warp and a
@@ -292,10 +329,10 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
   int parity = 0;
   double* sums = s_sum[0];
 
-  // Sum over the vocabulary of r with the rejections of s_h applied.  All
-  // threads of the cluster call it; every one gets the same sum.  sums: the
-  // segments' sums; s_batch: those of this CTA's batches.
-  auto vocab_sum = [&](const float* p, const float* d, bool dist) -> double {
+  // Sums over the vocabulary of r with the rejections of s_h applied: `sums` gets
+  // every segment's, s_batch those of this CTA's batches.  All threads of the
+  // cluster call it; afterwards no warp of the CTA reads s_h any more.
+  auto vocab_sums = [&](const float* p, const float* d, bool dist) {
     double acc = 0.0;
     const bool vec = vec_p && (!dist || vec_d);
     for (int b = 0; b < n_batch; ++b) {
@@ -303,8 +340,8 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
       double one = 0.0;
       for (int y = y0 + b * batch; y < end; y += step) {
         double w[GROUPS][4];
-        if (dist) weights<true, GROUPS>(s_h, p, d, y + 4 * lane, y1, vec, w);
-        else weights<false, GROUPS>(s_h, p, d, y + 4 * lane, y1, vec, w);
+        if (dist) weights<true, GROUPS, 128>(s_h, p, d, y, y + 4 * lane, y1, vec, w);
+        else weights<false, GROUPS, 128>(s_h, p, d, y, y + 4 * lane, y1, vec, w);
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) one += (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
       }
@@ -317,11 +354,12 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
     if (lane < C) cluster.map_shared_rank(sums, lane)[seg] = acc;
     cluster.sync();
     parity ^= 1;   // the other buffer next: a CTA may still be reading this one
-    double all = 0.0;
-    for (int k = lane; k < n_seg; k += 32) all += sums[k];
+  };
+  const int per = (n_seg + 31) / 32;   // segment sums a lane looks at
+  auto lane_sums = [&](double* v) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    return all;
+    for (int k = 0; k < VF_PER_LANE; ++k)
+      v[k] = k < per && lane * per + k < n_seg ? sums[lane * per + k] : 0.0;
   };
 
   // ---- the walk, by the first warp of every CTA; the others join for a sum
@@ -402,10 +440,14 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
     __syncthreads();
     c = s_node;
     if (!s_sum_wanted) break;
-    const double z = vocab_sum(a.probs + (size_t)(q0 + c) * a.ld_p,
-                               a.draft_probs + (size_t)s_drow[c] * a.ld_d, true);
+    vocab_sums(a.probs + (size_t)(q0 + c) * a.ld_p, a.draft_probs + (size_t)s_drow[c] * a.ld_d,
+               true);
     // (past the cluster's barrier no warp of this CTA reads s_h or the command)
     if (warp == 0) {
+      double z = 0.0;
+      for (int k = lane; k < n_seg; k += 32) z += sums[k];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
       if (lane == 0) s_h.inv_z[s_h.n - 1] = z > 0.0 ? 1.0 / z : 0.0;
       __syncwarp();
       unscaled = false;
@@ -417,89 +459,50 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
   const float* prow = a.probs + (size_t)(q0 + c) * a.ld_p;
   const bool dist = s_drow[c] >= 0;
   const float* drow = dist ? a.draft_probs + (size_t)s_drow[c] * a.ld_d : nullptr;
-  double total = vocab_sum(prow, drow, dist);
-  if (dist && s_h.n > 0 && !(total > 0.0)) {
+  vocab_sums(prow, drow, dist);
+  // the segment (the same answer in every warp of the cluster), its batch, then the
+  // element; a target that rounding leaves past a level's last sum takes the last
+  // positive value
+  double at = s_u[0], total, v[VF_PER_LANE];
+  lane_sums(v);
+  int found = locate<VF_PER_LANE>(v, true, at, total);
+  if (found < 0 && dist && s_h.n > 0) {
     __syncthreads();
     if (tid == 0) s_h.inv_z[s_h.n - 1] = 0.0;
     __syncthreads();
-    total = vocab_sum(prow, drow, dist);
+    vocab_sums(prow, drow, dist);
+    at = s_u[0];
+    lane_sums(v);
+    found = locate<VF_PER_LANE>(v, true, at, total);
   }
   if (rank == 0 && warp == 0) {
     for (int k = n + lane; k < t.path_w; k += 32) path[k] = -1;
     if (lane == 0) {
       t.n_accepted[seq] = n - 1;
-      if (!(total > 0.0)) t.next_ids[seq] = -1;
+      if (found < 0) t.next_ids[seq] = -1;
     }
   }
-  if (!(total > 0.0)) return;
-  // The CTA, its warp, its batch, then the element in which the cumulative sum
-  // passes the target.  Among the sums of a level (one a lane) that is the last
-  // positive one whose exclusive prefix does not exceed what is left of the
-  // target: some lane always qualifies, and every warp of the cluster picks the
-  // same one, however the prefixes are rounded.
-  double at = fmax((double)s_u[0] * total, 0.0);   // a NaN aims at 0
-  auto locate = [&](double v) -> int {
-    double inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    double ex = __shfl_up_sync(0xffffffffu, inc, 1);
-    if (lane == 0) ex = 0.0;
-    const int k = 31 - __clz(__ballot_sync(0xffffffffu, v > 0.0 && ex <= at));
-    at = k < 0 ? at : at - __shfl_sync(0xffffffffu, ex, k & 31);
-    return k;
-  };
-  double v = 0.0;
-  if (lane < C)
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k) v += sums[lane * WARPS + k];
-  if (locate(v) != rank) return;
-  if (locate(lane < WARPS ? sums[rank * WARPS + lane] : 0.0) != warp) return;
-  const int b = locate(lane < n_batch ? s_batch[warp][lane] : 0.0);
-  if (b < 0) return;
+  if (found < 0 || found / VF_PER_LANE * per + found % VF_PER_LANE != seg) return;
+  int b = 0;
+  if (n_batch > 1) {
+    const double one = lane < n_batch ? s_batch[warp][lane] : 0.0;
+    b = locate<1>(&one, false, at, total);
+    if (b < 0) return;     // (a positive segment has a positive batch)
+  }
+  // a lane's 4 * GROUPS elements are neighbours now
   const bool vec = vec_p && (!dist || vec_d);
   const int end = min(y0 + (b + 1) * batch, y1);
-  double run = 0.0;
   int next = -1;
   for (int y = y0 + b * batch; y < end; y += step) {
-    double w[GROUPS][4], inc[GROUPS];
-    if (dist) weights<true, GROUPS>(s_h, prow, drow, y + 4 * lane, y1, vec, w);
-    else weights<false, GROUPS>(s_h, prow, drow, y + 4 * lane, y1, vec, w);
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) inc[g] = (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1)
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        const double up = __shfl_up_sync(0xffffffffu, inc[g], o);
-        if (lane >= o) inc[g] += up;
-      }
-    bool found = false;
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      double cum = __shfl_up_sync(0xffffffffu, inc[g], 1);
-      cum = run + (lane > 0 ? cum : 0.0);
-      int hit = -1, pos = -1;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        cum += w[g][e];
-        if (w[g][e] > 0.0) {
-          pos = y + 128 * g + 4 * lane + e;
-          if (hit < 0 && cum > at) hit = pos;
-        }
-      }
-      const unsigned any = __ballot_sync(0xffffffffu, hit >= 0);
-      const unsigned some = __ballot_sync(0xffffffffu, pos >= 0);
-      if (!found) {   // the first hit, or so far the last positive element
-        if (any) next = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
-        else if (some) next = __shfl_sync(0xffffffffu, pos, 31 - __clz(some));
-        found = any != 0;
-      }
-      run += __shfl_sync(0xffffffffu, inc[g], 31);
-    }
-    if (found) break;
+    double w[GROUPS][4];
+    const int mine = y + lane * 4 * GROUPS;
+    if (dist) weights<true, GROUPS, 4>(s_h, prow, drow, y, mine, y1, vec, w);
+    else weights<false, GROUPS, 4>(s_h, prow, drow, y, mine, y1, vec, w);
+    const double left = at;
+    const int e = locate<4 * GROUPS>(&w[0][0], false, at, total);
+    if (e >= 0) next = y + e;
+    if (left < total) break;
+    at = left - total;
   }
   if (lane == 0) t.next_ids[seq] = next;
 }
