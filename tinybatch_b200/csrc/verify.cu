@@ -143,10 +143,23 @@ __device__ __forceinline__ double residual(const Rejections& h, bool dist, int t
   return r;
 }
 
+// Whether one of the rejected tokens lies in first .. first+count-1 (all lanes of
+// the warp ask the same).
 __device__ __forceinline__ bool rejected(const Rejections& h, int first, int count) {
   bool s = false;
-  for (int k = 0; k < h.n; ++k) s |= (unsigned)(h.token[k] - first) < (unsigned)count;
-  return s;
+  for (int k0 = 0; k0 < h.n; k0 += 32) {
+    const int k = k0 + (threadIdx.x & 31);
+    s |= k < h.n && (unsigned)(h.token[k] - first) < (unsigned)count;
+  }
+  return __any_sync(0xffffffffu, s);
+}
+
+// Eight bytes into a cluster member's shared memory, counted by its mbarrier.
+__device__ __forceinline__ void st_async_f64(uint32_t addr, double v, uint32_t bar) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(addr),
+      "l"(__double_as_longlong(v)), "r"(bar)
+      : "memory");
 }
 
 __device__ __forceinline__ float4 load4(const float* row, int y, int end, bool vec) {
@@ -156,11 +169,13 @@ __device__ __forceinline__ float4 load4(const float* row, int y, int end, bool v
 }
 
 // r of tokens y + STRIDE g .. + 3, g < GROUPS (y already the lane's, base the
-// warp's; 0 from `end` on).  All loads are issued before the first is used.
+// warp's; 0 from `end` on); dv: their draft probabilities, 0 for rejected tokens.
+// All loads are issued before the first is used.
 template <bool DIST, int GROUPS, int STRIDE>
 __device__ __forceinline__ void weights(const Rejections& h, const float* p, const float* d,
-                                        int base, int y, int end, bool vec, double (*w)[4]) {
-  float4 pv[GROUPS], dv[GROUPS];
+                                        int base, int y, int end, bool vec, double (*w)[4],
+                                        float4* dv) {
+  float4 pv[GROUPS];
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) pv[g] = load4(p, y + STRIDE * g, end, vec);
   if (DIST)
@@ -250,7 +265,8 @@ __device__ __forceinline__ int locate(const double* v, bool fraction, double& at
 // vocabulary: one for each rejection whose Z a later sibling's test needs, one
 // for the sample.
 // GROUPS: 128-token groups whose loads a warp has in flight.
-template <int THREADS, int MIN_CTAS, int GROUPS>
+// KEEP: a warp keeps its segment's r between the passes at a node where one step covers it.
+template <int THREADS, int MIN_CTAS, int GROUPS, bool KEEP>
 __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyArgs a) {
   namespace cg = cooperative_groups;
   constexpr int WARPS = THREADS / 32;
@@ -259,7 +275,8 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
   __shared__ float s_p[VF_NODES], s_d[VF_NODES], s_u[VF_NODES];
   __shared__ Rejections s_h;
   __shared__ int s_node, s_sum_wanted;
-  __shared__ double s_sum[2][VF_MAX_CLUSTER * WARPS];
+  __shared__ double s_sum[2][VF_MAX_CLUSTER * WARPS + 32];   // padded: see `pad`
+  __shared__ uint64_t s_arrived[2];
   __shared__ double s_batch[WARPS][VF_BATCHES];
   cg::cluster_group cluster = cg::this_cluster();
   pdl_wait();
@@ -282,6 +299,12 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
     }
     return;
   }
+  if (tid == 0) {
+    mbar_init(&s_arrived[0], 1);
+    mbar_init(&s_arrived[1], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
   auto started = cluster.barrier_arrive();   // waited for before the first remote store
 
   // ---- the tree and, for every node, the probabilities its test compares
@@ -326,22 +349,55 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
   const int y1 = (int)min(y_begin + (long long)n_batch * batch, (long long)a.vocab);
   const bool vec_p = a.ld_p % 4 == 0 && reinterpret_cast<uintptr_t>(a.probs) % 16 == 0;
   const bool vec_d = a.ld_d % 4 == 0 && reinterpret_cast<uintptr_t>(a.draft_probs) % 16 == 0;
-  int parity = 0;
-  double* sums = s_sum[0];
+  const int log_per = n_seg > 32 ? 31 - __clz(n_seg / 32) : 0;   // (n_seg is a power of two)
+  auto pad = [&](int i) { return i + (i >> log_per); };   // a lane's run of sums has no bank to share
+  int pass = 0;
+  bool lost = false;                 // a wait ran out (the status says so): no further waits
+  const double* sums = s_sum[0];
+  double w[GROUPS][4];               // r of a step, and d where it is not rejected
+  float4 dv[GROUPS];
+  int held = -1, applied = 0;        // KEEP: the node and rejections they stand for
 
-  // Sums over the vocabulary of r with the rejections of s_h applied: `sums` gets
-  // every segment's, s_batch those of this CTA's batches.  All threads of the
-  // cluster call it; afterwards no warp of the CTA reads s_h any more.
-  auto vocab_sums = [&](const float* p, const float* d, bool dist) {
+  // Sums over the vocabulary of r with the rejections of s_h applied, at node c:
+  // `sums` gets every segment's, s_batch those of this CTA's batches.  All threads of
+  // the cluster call it; no warp of the CTA reads s_h from the moment all sums have
+  // arrived.  Every sum travels as an asynchronous store counted by the receiver's
+  // barrier (a cluster barrier costs twice as much); two buffers take turns: a CTA is
+  // at most one pass ahead, since a pass needs every CTA's sums.
+  auto vocab_sums = [&](int c, bool dist) {
+    const float* p = a.probs + (size_t)(q0 + c) * a.ld_p;
+    const float* d = dist ? a.draft_probs + (size_t)s_drow[c] * a.ld_d : nullptr;
     double acc = 0.0;
     const bool vec = vec_p && (!dist || vec_d);
+    bool have = KEEP && dist && held == c;
+    if (have) {
+      // fold in the last rejection's Z, apply the new one
+      for (; applied < s_h.n; ++applied) {
+        const double iz = applied > 0 ? s_h.inv_z[applied - 1] : 1.0, sc = s_h.scale[applied];
+        if (iz == 0.0) break;        // a rejection that was taken back: start over
+        const int x = s_h.token[applied] - y0 - 4 * lane;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          w[g][0] = fmax(w[g][0] * iz - dv[g].x * sc, 0.0);
+          w[g][1] = fmax(w[g][1] * iz - dv[g].y * sc, 0.0);
+          w[g][2] = fmax(w[g][2] * iz - dv[g].z * sc, 0.0);
+          w[g][3] = fmax(w[g][3] * iz - dv[g].w * sc, 0.0);
+          if (x == 128 * g) dv[g].x = 0.f;
+          if (x == 128 * g + 1) dv[g].y = 0.f;
+          if (x == 128 * g + 2) dv[g].z = 0.f;
+          if (x == 128 * g + 3) dv[g].w = 0.f;
+        }
+      }
+      have = applied == s_h.n && (s_h.n == 0 || s_h.inv_z[s_h.n - 1] != 0.0);
+    }
     for (int b = 0; b < n_batch; ++b) {
       const int end = min(y0 + (b + 1) * batch, y1);
       double one = 0.0;
       for (int y = y0 + b * batch; y < end; y += step) {
-        double w[GROUPS][4];
-        if (dist) weights<true, GROUPS, 128>(s_h, p, d, y, y + 4 * lane, y1, vec, w);
-        else weights<false, GROUPS, 128>(s_h, p, d, y, y + 4 * lane, y1, vec, w);
+        if (!have) {
+          if (dist) weights<true, GROUPS, 128>(s_h, p, d, y, y + 4 * lane, y1, vec, w, dv);
+          else weights<false, GROUPS, 128>(s_h, p, d, y, y + 4 * lane, y1, vec, w, dv);
+        }
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) one += (w[g][0] + w[g][1]) + (w[g][2] + w[g][3]);
       }
@@ -350,16 +406,31 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
       if (lane == 0) s_batch[warp][b] = one;
       acc += one;
     }
-    sums = s_sum[parity];
-    if (lane < C) cluster.map_shared_rank(sums, lane)[seg] = acc;
-    cluster.sync();
-    parity ^= 1;   // the other buffer next: a CTA may still be reading this one
+    if (KEEP && !have) {
+      // held from now on where one step is the whole segment (the last entry's
+      // inv_z, still 1, has not been folded in)
+      held = dist && n_batch * batch == step && s_h.n > 0 && s_h.inv_z[s_h.n - 1] == 1.0 ? c : -1;
+      applied = s_h.n;
+    }
+    const int buf = pass & 1;
+    sums = s_sum[buf];
+    if (C > 1) {
+      if (tid == 0) mbar_arrive_expect_tx(&s_arrived[buf], n_seg * 8);
+      if (lane < C)
+        st_async_f64(cluster_map(smem_u32(&s_sum[buf][pad(seg)]), lane), acc,
+                     cluster_map(smem_u32(&s_arrived[buf]), lane));
+      if (!lost) lost = !mbar_wait(&s_arrived[buf], (pass >> 1) & 1);
+    } else if (lane == 0) {   // (asynchronous stores are for clusters: without one they are refused)
+      s_sum[buf][pad(seg)] = acc;
+    }
+    ++pass;
+    __syncthreads();
   };
   const int per = (n_seg + 31) / 32;   // segment sums a lane looks at
   auto lane_sums = [&](double* v) {
 #pragma unroll
     for (int k = 0; k < VF_PER_LANE; ++k)
-      v[k] = k < per && lane * per + k < n_seg ? sums[lane * per + k] : 0.0;
+      v[k] = k < per && lane * per + k < n_seg ? sums[pad(lane * per + k)] : 0.0;
   };
 
   // ---- the walk, by the first warp of every CTA; the others join for a sum
@@ -440,12 +511,10 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
     __syncthreads();
     c = s_node;
     if (!s_sum_wanted) break;
-    vocab_sums(a.probs + (size_t)(q0 + c) * a.ld_p, a.draft_probs + (size_t)s_drow[c] * a.ld_d,
-               true);
-    // (past the cluster's barrier no warp of this CTA reads s_h or the command)
+    vocab_sums(c, true);
     if (warp == 0) {
       double z = 0.0;
-      for (int k = lane; k < n_seg; k += 32) z += sums[k];
+      for (int k = lane; k < n_seg; k += 32) z += sums[pad(k)];
 #pragma unroll
       for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
       if (lane == 0) s_h.inv_z[s_h.n - 1] = z > 0.0 ? 1.0 / z : 0.0;
@@ -459,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
   const float* prow = a.probs + (size_t)(q0 + c) * a.ld_p;
   const bool dist = s_drow[c] >= 0;
   const float* drow = dist ? a.draft_probs + (size_t)s_drow[c] * a.ld_d : nullptr;
-  vocab_sums(prow, drow, dist);
+  vocab_sums(c, dist);
   // the segment (the same answer in every warp of the cluster), its batch, then the
   // element; a target that rounding leaves past a level's last sum takes the last
   // positive value
@@ -470,7 +539,7 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
     __syncthreads();
     if (tid == 0) s_h.inv_z[s_h.n - 1] = 0.0;
     __syncthreads();
-    vocab_sums(prow, drow, dist);
+    vocab_sums(c, dist);
     at = s_u[0];
     lane_sums(v);
     found = locate<VF_PER_LANE>(v, true, at, total);
@@ -482,6 +551,8 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
       if (found < 0) t.next_ids[seq] = -1;
     }
   }
+  // (a CTA that gave up waiting stays until nobody can still write to it)
+  if (lost) asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
   if (found < 0 || found / VF_PER_LANE * per + found % VF_PER_LANE != seg) return;
   int b = 0;
   if (n_batch > 1) {
@@ -494,10 +565,9 @@ __global__ void __launch_bounds__(THREADS, MIN_CTAS) verify_kernel(const VerifyA
   const int end = min(y0 + (b + 1) * batch, y1);
   int next = -1;
   for (int y = y0 + b * batch; y < end; y += step) {
-    double w[GROUPS][4];
     const int mine = y + lane * 4 * GROUPS;
-    if (dist) weights<true, GROUPS, 4>(s_h, prow, drow, y, mine, y1, vec, w);
-    else weights<false, GROUPS, 4>(s_h, prow, drow, y, mine, y1, vec, w);
+    if (dist) weights<true, GROUPS, 4>(s_h, prow, drow, y, mine, y1, vec, w, dv);
+    else weights<false, GROUPS, 4>(s_h, prow, drow, y, mine, y1, vec, w, dv);
     const double left = at;
     const int e = locate<4 * GROUPS>(&w[0][0], false, at, total);
     if (e >= 0) next = y + e;
@@ -541,14 +611,14 @@ int verify_launch(const VerifyArgs& a, int max_q, cudaStream_t st) {
   if (n > 0x7fffffff / VF_MAX_CLUSTER) return arg_err("n_seqs");
   if (n * 16 <= 148) {
     static std::atomic<unsigned long long> devs{0};
-    if (int rc = wide_cluster_once(verify_kernel<512, 1, 5>, devs, "verification cluster attribute"))
+    if (int rc = wide_cluster_once(verify_kernel<512, 1, 5, true>, devs, "verification cluster attribute"))
       return rc;
-    return launch_pdl(verify_kernel<512, 1, 5>, dim3(n * 16), dim3(512), 0, st, 16,
+    return launch_pdl(verify_kernel<512, 1, 5, true>, dim3(n * 16), dim3(512), 0, st, 16,
                       "draft verification launch", a);
   }
   int cluster = 8;
   while (cluster > 1 && n * (long long)cluster > 148 * 4) cluster /= 2;
-  return launch_pdl(verify_kernel<256, 4, 2>, dim3(n * cluster), dim3(256), 0, st, cluster,
+  return launch_pdl(verify_kernel<256, 4, 2, false>, dim3(n * cluster), dim3(256), 0, st, cluster,
                     "draft verification launch", a);
 }
 
