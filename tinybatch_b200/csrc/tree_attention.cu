@@ -166,9 +166,9 @@ static int tree_simple_launch(const TreeAttnArgs& t, cudaStream_t st) {
 //              lanes issue a tile's boxes.  Other block sizes: 16-byte cp.async pieces into the same layout, every key looking up its
 //              block (a third slower).  K and V have rings of their own: a K stage
 //              is free once its S is done, before the V that came with it
-//   warp 5     MMA issue: S of the next tile goes into the other S buffer while
-//              the softmax works on this one; P (bf16) overwrites S in place and
-//              is read from TMEM
+//   warp 5     MMA issue.  P (bf16) has two buffers of its own in TMEM, so S of the
+//              next tile follows as soon as the softmax has S in registers and is
+//              there when it has written P
 // O is accumulated in TMEM; a row's exponent reference moves only when its
 // maximum has grown by more than TT_RESCALE (log2 units), as in the prefill kernel.
 // Two CTAs an SM: one's chain S -> softmax -> P V, its start and its end hide
@@ -205,6 +205,7 @@ struct TreeTcLayout {
   static constexpr int OFF_BAR = DATA;
   static constexpr int N_BARS = 4 * MAX_STAGES + 7;
   static constexpr int SMEM = OFF_BAR + 512 + 512;     // barriers; alignment slack
+  static constexpr uint32_t COL_P = TT_KEYS;           // two buffers of TT_KEYS / 2 columns
   static constexpr uint32_t COL_O = 2 * TT_KEYS;
   static constexpr uint32_t TMEM_COLS = 256;
   __device__ static constexpr int q_half(int act) { return act * 4096; }   // 32 rows a warp
@@ -220,7 +221,7 @@ struct TreeTcLayout {
                 "merge tables");
   static_assert(N_BARS * 8 + 12 <= 512, "barrier area");
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
-  static_assert(2 * TT_KEYS + HD <= 256, "TMEM: two S buffers and O in half of it");
+  static_assert(2 * TT_KEYS + HD <= 256, "TMEM: S, two P buffers and O in half of it");
 };
 
 // Position in a ring of n stages; `phase` flips with every lap.
@@ -252,6 +253,17 @@ __device__ __forceinline__ void st_cluster_f2(uint32_t addr, float x, float y) {
 }
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t x) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
+}
+
+// True in one lane of the (converged) warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 // Bits of a word whose bf16 halves are infinite or NaN (those halves all ones).
@@ -363,7 +375,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   uint64_t* k_empty = k_full + L::MAX_STAGES;
   uint64_t* v_full = k_empty + L::MAX_STAGES;
   uint64_t* v_empty = v_full + L::MAX_STAGES;
-  uint64_t* s_full = v_empty + L::MAX_STAGES;                       // [2]
+  uint64_t* s_full = v_empty + L::MAX_STAGES;
+  uint64_t* s_free = s_full + 1;                                    // S is in registers
   uint64_t* p_full = s_full + 2;                                    // [2]
   uint64_t* pv_done = p_full + 2;                                   // [2]
   uint64_t* q_full = pv_done + 2;
@@ -388,10 +401,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     // full and empty barriers of K, then of V, then the S and P V ones
     if (lane < 4 * L::MAX_STAGES)
       mbar_init(&k_full[lane], !TMA && (lane / L::MAX_STAGES) % 2 == 0 ? 32 : 1);
-    if (lane < 2) {
-      mbar_init(&s_full[lane], 1);
-      mbar_init(&pv_done[lane], 1);
-    }
+    if (lane < 2) mbar_init(&pv_done[lane], 1);
+    if (lane == 0) mbar_init(s_full, 1);
     fence_mbar_init();
     if (TMA && lane == 0) prefetch_tmap(&map);
     __syncwarp();
@@ -494,6 +505,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   };
   if (warp == 4 && lane == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&p_full[i], 32 * act);
+    mbar_init(s_free, 32 * act);
     mbar_init(q_full, 32 * act);
     *s_bad = 0;
     fence_mbar_init();
@@ -564,49 +576,62 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       cp_wait<0>();   // nothing in flight at exit
     }
   } else if (warp == 5) {
-    // ---------------- MMA issue
-    if (lane == 0 && nt > 0) {
+    // ---------------- MMA issue: the whole warp walks the loop, one elected lane issues.
+    // Control flow and descriptors stay warp-uniform that way (in uniform registers);
+    // with a single lane in the loop an MMA took ~110 cycles to issue and the issue
+    // bounded the kernel
+    if (nt > 0) {
       constexpr uint32_t idesc_s = idesc_bf16_m128(TT_KEYS);
       constexpr uint32_t idesc_o = idesc_bf16_m128(HD) | (1u << 16);   // V: MN-major
+      const bool lead = elect_one();
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
+      };
       RingPos kp, vp;
       auto issue_s = [&](int j) -> bool {
-        if (!mbar_wait(&k_full[kp.st], kp.phase)) return false;
+        if (!wait(&k_full[kp.st], kp.phase)) return false;
         tc_fence_after();
         if (!TMA) fence_proxy_async_smem();   // K arrived through the generic proxy
         const uint32_t kb = sbase + off_k + kp.st * L::STAGE;
+        if (lead) {
 #pragma unroll
-        for (int h = 0; h < L::HALVES; ++h)
+          for (int h = 0; h < L::HALVES; ++h)
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_bf16(tmem + (j & 1) * TT_KEYS, sw128_desc(sbase + h * q_half + kk * 32),
-                        sw128_k_desc(kb + h * 1024 + kk * 32, L::GROUP), idesc_s,
-                        (h | kk) ? 1u : 0u);
-        tc_commit(&s_full[j & 1]);
-        tc_commit(&k_empty[kp.st]);
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_bf16(tm, sw128_desc(sbase + h * q_half + kk * 32),
+                          sw128_k_desc(kb + h * 1024 + kk * 32, L::GROUP), idesc_s,
+                          (h | kk) ? 1u : 0u);
+          tc_commit(s_full);
+          tc_commit(&k_empty[kp.st]);
+        }
+        __syncwarp();
         kp.next(KS);
         return true;
       };
-      bool good = mbar_wait(q_full, 0);
+      bool good = wait(q_full, 0);
       if (good) good = issue_s(0);
       for (int j = 0; j < nt && good; ++j) {
         if (j + 1 < nt) {
-          // S of the next tile overwrites P of the previous one
-          if (j > 0) good = mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);
+          good = wait(s_free, j & 1);
           if (good) good = issue_s(j + 1);
           if (!good) break;
         }
-        if (!mbar_wait(&v_full[vp.st], vp.phase)) break;
-        if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1)) break;
+        if (!wait(&v_full[vp.st], vp.phase)) break;
+        if (!wait(&p_full[j & 1], (j >> 1) & 1)) break;
         tc_fence_after();
         if (!TMA) fence_proxy_async_smem();   // V too
         const uint32_t vb = sbase + off_v + vp.st * L::STAGE;
+        if (lead) {
 #pragma unroll
-        for (int ks = 0; ks < TT_KEYS / 16; ++ks)
-          tc_mma_bf16_ts(tmem + L::COL_O, tmem + (j & 1) * TT_KEYS + ks * 8,
-                         sw128_mn_desc(vb + ks * 2 * L::GROUP, 1024, L::GROUP), idesc_o,
-                         (j | ks) ? 1u : 0u);
-        tc_commit(&v_empty[vp.st]);
-        tc_commit(&pv_done[j & 1]);
+          for (int ks = 0; ks < TT_KEYS / 16; ++ks)
+            tc_mma_bf16_ts(tm + L::COL_O, tm + L::COL_P + (j & 1) * (TT_KEYS / 2) + ks * 8,
+                           sw128_mn_desc(vb + ks * 2 * L::GROUP, 1024, L::GROUP), idesc_o,
+                           (j | ks) ? 1u : 0u);
+          tc_commit(&v_empty[vp.st]);
+          tc_commit(&pv_done[j & 1]);
+        }
+        __syncwarp();
         vp.next(VS);
       }
     }
@@ -639,11 +664,14 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
     int done = 0;
     for (int j = 0; j < nt; ++j) {
       const int k0 = (t0 + j) * TT_KEYS;
-      const uint32_t ts = tmem + (j & 1) * TT_KEYS + lane_off;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], (j >> 1) & 1))) break;
+      const uint32_t ts = tmem + lane_off;
+      const uint32_t tp = tmem + L::COL_P + (j & 1) * (TT_KEYS / 2) + lane_off;
+      if (!__all_sync(0xffffffffu, mbar_wait(s_full, j & 1))) break;
       tc_fence_after();
       float x[TT_KEYS];
       tmem_ld64(ts, x);
+      tc_fence_before();
+      mbar_arrive(s_free);
       if (k0 + TT_KEYS > s.base) {                 // drafts, or places past the context
         const unsigned long long w = tree_window(m, k0, s.base, s.ctx);
         const uint32_t wl = (uint32_t)w, wh = (uint32_t)(w >> 32);
@@ -699,6 +727,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       const float mu = ref == -INFINITY ? 0.f : ref;
       const float2 sc2 = make_float2(sc, sc), nmu2 = make_float2(-mu, -mu);
       float2 sum2 = make_float2(0.f, 0.f);
+      // P V of two tiles before has read this P buffer
+      if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[j & 1], ((j - 2) >> 1) & 1))) break;
 #pragma unroll
       for (int c0 = 0; c0 < TT_KEYS; c0 += 32) {
         uint32_t w[16];
@@ -709,7 +739,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
           sum2 = add2(sum2, pv);
           w[e >> 1] = pack_bf16x2(pv.x, pv.y);
         }
-        tmem_st16(ts + (c0 >> 1), w);
+        tmem_st16(tp + (c0 >> 1), w);
       }
       tmem_wait_st();
       l += sum2.x + sum2.y;
