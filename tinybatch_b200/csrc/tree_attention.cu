@@ -272,24 +272,22 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
          ((w & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u);
 }
 
-// Which of the keys k0 .. k0+63 a row sees (base: first draft's position).
-__device__ __forceinline__ unsigned long long tree_window(const unsigned long long* m, int k0,
-                                                          int base, int ctx) {
+// Which of the keys k0 .. k0+63 a row sees (base: first draft's position).  m0: its
+// first mask word; the others (trees of more than 64 nodes) are read when needed.
+__device__ __forceinline__ unsigned long long tree_window(const unsigned long long* mask, int words,
+                                                          unsigned long long m0, int k0, int base,
+                                                          int ctx) {
   const int d = k0 - base;
   unsigned long long w;
   if (d <= -64) {
     w = ~0ull;
   } else if (d < 0) {
-    w = ((1ull << -d) - 1) | (m[0] << -d);
+    w = ((1ull << -d) - 1) | (m0 << -d);
   } else {
     const int k = d >> 6, o = d & 63;
-    unsigned long long lo = 0, hi = 0;
-#pragma unroll
-    for (int i = 0; i < TREE_WORDS; ++i) {
-      if (i == k) lo = m[i];
-      if (i == k + 1) hi = m[i];
-    }
-    w = o ? (lo >> o) | (hi << (64 - o)) : lo;
+    const unsigned long long lo = k == 0 ? m0 : k < words ? mask[k] : 0ull;
+    w = lo >> o;
+    if (o && k + 1 < words) w |= mask[k + 1] << (64 - o);
   }
   const int left = ctx - k0;
   if (left < 64) w &= left > 0 ? (1ull << left) - 1 : 0ull;
@@ -362,8 +360,11 @@ __device__ __forceinline__ void merge_rows(const uint8_t* smem, const float2* s_
   }
 }
 
+// (at most 128 registers: four warps of each scheduler's, so that a CTA can follow
+// another as soon as it ends.  Six warps of 168 fitted twice, but with the four that
+// TMEM ties to their schedulers a new CTA then waited for an empty SM)
 template <int HD, bool TMA>
-__global__ void __launch_bounds__(TT_THREADS, 2)
+__global__ void __launch_bounds__(256, 2)
     tree_attn_tc_kernel(const __grid_constant__ CUtensorMap map, const TreeAttnArgs t,
                         const int row_tiles) {
   using L = TreeTcLayout<HD>;
@@ -520,7 +521,6 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
   const int R = rt * TT_ROWS + (valid ? r : 0), node = div_group(t, R);
   const size_t row = (size_t)s.q0 + node;
   const int col = (kvh * G + R - node * G) * HD;   // the row's place in q and out
-  unsigned long long m[TREE_WORDS] = {0, 0, 0, 0};
   const uint32_t tmem = *tmem_slot;
   float ref = -INFINITY, l = 0.f;                  // a row's exponent reference (log2) and sum
 
@@ -652,9 +652,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       }
       cp_commit();
     }
-#pragma unroll
-    for (int i = 0; i < TREE_WORDS; ++i)
-      if (i < t.mask_w && valid) m[i] = t.mask[row * t.mask_ld + i];
+    const unsigned long long* mask = t.mask + row * t.mask_ld;   // (a missing row masks as row 0)
+    const unsigned long long m0 = mask[0];
     cp_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(q_full);
@@ -668,18 +667,29 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
       const uint32_t tp = tmem + L::COL_P + (j & 1) * (TT_KEYS / 2) + lane_off;
       if (!__all_sync(0xffffffffu, mbar_wait(s_full, j & 1))) break;
       tc_fence_after();
+      constexpr int KH = TT_KEYS / 2;
       float x[TT_KEYS];
       tmem_ld64(ts, x);
       tc_fence_before();
-      mbar_arrive(s_free);
-      if (k0 + TT_KEYS > s.base) {                 // drafts, or places past the context
-        const unsigned long long w = tree_window(m, k0, s.base, s.ctx);
-        const uint32_t wl = (uint32_t)w, wh = (uint32_t)(w >> 32);
+      mbar_arrive(s_free);                         // S of the next tile may overwrite it
+      const bool edge = k0 + TT_KEYS > s.base;     // drafts, or places past the context
+      if (edge) {
+        const unsigned long long win = tree_window(mask, t.mask_w, m0, k0, s.base, s.ctx);
+        const uint32_t wl = (uint32_t)win, wh = (uint32_t)(win >> 32);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < KH; ++e) {
           if (!(wl & (1u << e))) x[e] = -INFINITY;
-          if (!(wh & (1u << e))) x[32 + e] = -INFINITY;
+          if (!(wh & (1u << e))) x[KH + e] = -INFINITY;
         }
+      }
+      float mx = fmax3(x[0], x[1], x[2]), mx2 = fmax3(x[3], x[4], x[5]);
+#pragma unroll
+      for (int e = 6; e + 3 < TT_KEYS; e += 4) {   // two chains
+        mx = fmax3(mx, x[e], x[e + 1]);
+        mx2 = fmax3(mx2, x[e + 2], x[e + 3]);
+      }
+      mx = fmaxf(fmax3(mx, x[TT_KEYS - 2], x[TT_KEYS - 1]), mx2);
+      if (edge) {
         const int lap = j / VS, st = j - lap * VS;
         if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], lap & 1))) break;
         uint8_t* vb = smem + off_v + st * L::STAGE;
@@ -702,9 +712,6 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
         }
         fence_proxy_async_smem();
       }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < TT_KEYS; e += 2) mx = fmax3(mx, x[e], x[e + 1]);
       mx *= sc;
       const bool move = mx > ref + TT_RESCALE;     // any finite max when ref is -inf
       const bool rescale = move && ref != -INFINITY;
@@ -714,35 +721,40 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
         if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1))) break;
         tc_fence_after();
 #pragma unroll
-        for (int c0 = 0; c0 < HD; c0 += 32) {
-          float v[32];
-          tmem_ld32(to + c0, v);
+        for (int c0 = 0; c0 < HD; c0 += 16) {
+          float v[16];
+          tmem_ld16(to + c0, v);
+          uint32_t u[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] *= alpha;
-          tmem_st32(to + c0, v);
+          for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(v[e] * alpha);
+          tmem_st16(to + c0, u);
         }
       }
       if (move) ref = mx;
       l *= alpha;
       const float mu = ref == -INFINITY ? 0.f : ref;
       const float2 sc2 = make_float2(sc, sc), nmu2 = make_float2(-mu, -mu);
-      float2 sum2 = make_float2(0.f, 0.f);
+      float2 sum2 = make_float2(0.f, 0.f), sum3 = sum2;
       // P V of two tiles before has read this P buffer
       if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[j & 1], ((j - 2) >> 1) & 1))) break;
 #pragma unroll
-      for (int c0 = 0; c0 < TT_KEYS; c0 += 32) {
-        uint32_t w[16];
+      for (int c0 = 0; c0 < TT_KEYS; c0 += KH) {
+        uint32_t w[KH / 2];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float2 xv = fma2(make_float2(x[c0 + e], x[c0 + e + 1]), sc2, nmu2);
-          const float2 pv = make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
-          sum2 = add2(sum2, pv);
-          w[e >> 1] = pack_bf16x2(pv.x, pv.y);
+        for (int e = 0; e < KH; e += 4) {
+          const float2 xa = fma2(make_float2(x[c0 + e], x[c0 + e + 1]), sc2, nmu2);
+          const float2 xb = fma2(make_float2(x[c0 + e + 2], x[c0 + e + 3]), sc2, nmu2);
+          const float2 pa = make_float2(ex2_approx(xa.x), ex2_approx(xa.y));
+          const float2 pb = make_float2(ex2_approx(xb.x), ex2_approx(xb.y));
+          sum2 = add2(sum2, pa);
+          sum3 = add2(sum3, pb);
+          w[e >> 1] = pack_bf16x2(pa.x, pa.y);
+          w[(e >> 1) + 1] = pack_bf16x2(pb.x, pb.y);
         }
         tmem_st16(tp + (c0 >> 1), w);
       }
       tmem_wait_st();
-      l += sum2.x + sum2.y;
+      l += (sum2.x + sum2.y) + (sum3.x + sum3.y);
       tc_fence_before();
       mbar_arrive(&p_full[j & 1]);
       done = j + 1;
