@@ -196,12 +196,15 @@ def _mat(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int | None, dev: 
             dev)
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream     # torch.cuda.current_stream without its object
+# torch.cuda.current_stream / current_device without their objects and checks
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_I32, _I64, _F32, _BF16 = torch.int32, torch.int64, torch.float32, torch.bfloat16
 
 
 def _run_on(dev: int, what: str, fn, *args) -> None:
     """Call ``fn(*args, stream)`` on device ``dev``'s current stream."""
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -226,34 +229,32 @@ def paged_attention_tree(q, out, kv_pool, *, n_q_heads, n_kv_heads, head_dim, bl
     lib = N.load()
     dev = _device(q)
     rows, n = len(q), len(ctx_len)
-    i32, bf = torch.int32, torch.bfloat16
-    qp, ldq, cols = _mat("q", q, bf, rows, dev)
-    op, ldo, ocols = _mat("out", out, bf, rows, dev)
+    qp, ldq, cols = _mat("q", q, _BF16, rows, dev)
+    op, ldo, ocols = _mat("out", out, _BF16, rows, dev)
     if cols != n_q_heads * head_dim or ocols != cols:
         raise ValueError(f"q and out: expected {n_q_heads * head_dim} columns, got {cols} and {ocols}")
     blocks = len(kv_pool)
-    pp = _vec("kv_pool", kv_pool, bf, (blocks, 2, n_kv_heads, block_size, head_dim), dev)
-    bp, ldb, width = _mat("block_tables", block_tables, i32, n, dev)
-    mp, ldm, words = _mat("tree_mask", tree_mask, torch.int64, rows, dev)
+    pp = _vec("kv_pool", kv_pool, _BF16, (blocks, 2, n_kv_heads, block_size, head_dim), dev)
+    bp, ldb, width = _mat("block_tables", block_tables, _I32, n, dev)
+    mp, ldm, words = _mat("tree_mask", tree_mask, _I64, rows, dev)
     seqs = (n,)
     _run_on(dev, "tb_paged_attention_tree", lib.tb_paged_attention_tree, qp, ldq, op, ldo, rows, pp,
             blocks, n_q_heads, n_kv_heads, head_dim, block_size, bp, ldb, width,
-            _vec("q_start", q_start, i32, seqs, dev), _vec("q_len", q_len, i32, seqs, dev),
-            _vec("ctx_len", ctx_len, i32, seqs, dev), n, mp, ldm, words,
+            _vec("q_start", q_start, _I32, seqs, dev), _vec("q_len", q_len, _I32, seqs, dev),
+            _vec("ctx_len", ctx_len, _I32, seqs, dev), n, mp, ldm, words,
             min(rows, 64 * words) if max_q is None else max_q, max_ctx, ctx_total)
 
 
 def _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev):
     """Sizes and pointers of the arguments both verifications share."""
-    i32 = torch.int32
     rows, seqs = ids.shape, q_len.shape
     if len(rows) != 1 or len(seqs) != 1:
         raise ValueError("ids and q_len: expected 1-d tensors")
     return (rows, seqs[0],
-            (_vec("ids", ids, i32, rows, dev), _vec("parents", parents, i32, rows, dev),
-             _vec("q_start", q_start, i32, seqs, dev), _vec("q_len", q_len, i32, seqs, dev)),
-            (_vec("n_accepted", n_accepted, i32, seqs, dev),
-             *_mat("path", path, i32, seqs[0], dev), _vec("next_ids", next_ids, i32, seqs, dev)))
+            (_vec("ids", ids, _I32, rows, dev), _vec("parents", parents, _I32, rows, dev),
+             _vec("q_start", q_start, _I32, seqs, dev), _vec("q_len", q_len, _I32, seqs, dev)),
+            (_vec("n_accepted", n_accepted, _I32, seqs, dev),
+             *_mat("path", path, _I32, seqs[0], dev), _vec("next_ids", next_ids, _I32, seqs, dev)))
 
 
 def verify_drafts_greedy(ids, parents, q_start, q_len, target_ids, n_accepted, path, next_ids, *,
@@ -266,7 +267,7 @@ def verify_drafts_greedy(ids, parents, q_start, q_len, target_ids, n_accepted, p
     lib = N.load()
     dev = _device(ids)
     rows, n, tree, outs = _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev)
-    tp = _vec("target_ids", target_ids, torch.int32, rows, dev)
+    tp = _vec("target_ids", target_ids, _I32, rows, dev)
     _run_on(dev, "tb_verify_drafts_greedy", lib.tb_verify_drafts_greedy, *tree, n, rows[0], max_q,
             tp, *outs)
 
@@ -285,17 +286,16 @@ def verify_drafts(ids, parents, q_start, q_len, probs, uniforms, n_accepted, pat
     lib = N.load()
     dev = _device(ids)
     rows, n, tree, outs = _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev)
-    f32 = torch.float32
-    pp, ldp, vocab = _mat("probs", probs, f32, rows[0], dev)
-    up = _vec("uniforms", uniforms, f32, rows, dev)
+    pp, ldp, vocab = _mat("probs", probs, _F32, rows[0], dev)
+    up = _vec("uniforms", uniforms, _F32, rows, dev)
     if (draft_probs is None) != (draft_rows is None):
         raise ValueError("draft_probs and draft_rows go together")
     draft = (None, 0, 0, None)
     if draft_probs is not None:
-        dp, ldd, cols = _mat("draft_probs", draft_probs, f32, None, dev)
+        dp, ldd, cols = _mat("draft_probs", draft_probs, _F32, None, dev)
         if cols != vocab:
             raise ValueError(f"draft_probs: expected {vocab} columns, got {cols}")
-        draft = (dp, ldd, len(draft_probs), _vec("draft_rows", draft_rows, torch.int32, rows, dev))
+        draft = (dp, ldd, len(draft_probs), _vec("draft_rows", draft_rows, _I32, rows, dev))
     _run_on(dev, "tb_verify_drafts", lib.tb_verify_drafts, *tree, n, rows[0], max_q, pp, ldp, vocab,
             *draft, up, *outs)
 
@@ -358,15 +358,14 @@ def keep_kv_path(pools, *, block_tables, q_len, ctx_len, path, n_accepted):
     lib = N.load()
     kv = _pools(pools)
     dev = kv.device
-    i32 = torch.int32
     seqs = q_len.shape
     if len(seqs) != 1:
         raise ValueError("q_len: expected a 1-d tensor")
     _run_on(dev, "tb_keep_kv_path", lib.tb_keep_kv_path, *kv.args,
-            *_mat("block_tables", block_tables, i32, seqs[0], dev),
-            _vec("q_len", q_len, i32, seqs, dev), _vec("ctx_len", ctx_len, i32, seqs, dev),
-            *_mat("path", path, i32, seqs[0], dev),
-            _vec("n_accepted", n_accepted, i32, seqs, dev), seqs[0])
+            *_mat("block_tables", block_tables, _I32, seqs[0], dev),
+            _vec("q_len", q_len, _I32, seqs, dev), _vec("ctx_len", ctx_len, _I32, seqs, dev),
+            *_mat("path", path, _I32, seqs[0], dev),
+            _vec("n_accepted", n_accepted, _I32, seqs, dev), seqs[0])
 
 
 def copy_kv_blocks(pools, pairs):
@@ -378,7 +377,7 @@ def copy_kv_blocks(pools, pairs):
     kv = _pools(pools)
     n = len(pairs)
     _run_on(kv.device, "tb_copy_kv_blocks", lib.tb_copy_kv_blocks, *kv.args,
-            _vec("pairs", pairs, torch.int32, (n, 2), kv.device), n)
+            _vec("pairs", pairs, _I32, (n, 2), kv.device), n)
 
 
 def embed(ids, emb, g, h, hg, sq):
