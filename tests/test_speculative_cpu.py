@@ -42,7 +42,8 @@ def attention(lib, **kw):
     (dict(ld_out=128), "ld_out"), (dict(words=0), "words"), (dict(words=5, mask_ld=5), "words"),
     (dict(words=2), "words"), (dict(max_q=65), "max_q"), (dict(max_q=-1), "max_q"), (dict(n=-1), "n_seqs"),
     (dict(n=70000), "65535"), (dict(q=None), "null pointer"), (dict(mask=None), "null pointer"),
-    (dict(ctx=None), "null pointer"), (dict(pool=P + 8), "aligned"), (dict(out=P + 2), "aligned")])
+    (dict(ctx=None), "null pointer"), (dict(pool=P + 8), "aligned"), (dict(out=P + 2), "aligned"),
+    (dict(mask=P + 4), "aligned")])
 def test_attention_argument_errors(lib, change, needle):
     assert attention(lib, **change) == 1
     assert needle in lib.tb_last_error().decode()

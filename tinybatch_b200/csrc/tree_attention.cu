@@ -44,7 +44,7 @@ __device__ __forceinline__ bool tree_seq(const TreeAttnArgs& t, int seq, TreeSeq
   s.base = s.ctx - s.ql;
   return s.ql >= 0 && s.ql <= t.max_q && s.ql <= 64 * t.mask_w && s.base >= 0 && s.q0 >= 0 &&
          s.q0 <= t.n_rows - s.ql &&
-         s.ctx <= (long long)t.bt_w * t.a.block_size;
+         s.ctx <= (long long)t.bt_w * t.a.block_size && s.ctx <= (1 << 30);
 }
 
 // ------------------------------------------------------------ short heads
@@ -922,6 +922,7 @@ int tree_attention(TreeAttnArgs t, int head_dim, int max_ctx, long long ctx_tota
     return arg_err("null pointer");
   for (const void* p : {(const void*)a.q, (const void*)a.out, (const void*)a.pool})
     if (reinterpret_cast<uintptr_t>(p) % 16) return arg_err("q / out / kv_pool must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(t.mask) % 8) return arg_err("tree_mask must be 8-byte aligned");
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   t.group = a.n_q_heads / a.n_kv_heads;
   t.group_magic = (unsigned)((0x100000000ull + t.group - 1) / t.group);
