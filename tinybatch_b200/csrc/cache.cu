@@ -8,7 +8,13 @@
 // nothing has to live on the device and a captured call keeps its own copy.
 //
 // Both kernels only move bytes: the floor is every moved byte read once and
-// written once.
+// written once.  Measured on a B200 (CUDA graph, inputs rotated through more than
+// the L2): 200 blocks of 64 KiB in 48 layers 147 us (629 MB written, 0.27 GB of
+// distinct sources read: 6.1 TB/s, 0.94 of the copy bandwidth); the accepted paths of
+// 64 sequences, 162 tokens in 48 layers, 16 us: 65 MB in runs of 256 bytes, all that
+// a pool keeps contiguous of a token and head, 4.0 TB/s.  More loads in flight a
+// thread, one wave of CTAs over several layers each, or fewer dependent loads before
+// the moves did not change the latter: the runs' scatter over DRAM pages bounds it.
 #include "common.cuh"
 #include "host.h"
 
@@ -128,7 +134,9 @@ __global__ void __launch_bounds__(KEEP_THREADS)
   if (col >= 2 * a.n_kv_heads * per_head) return;
   __nv_bfloat16* pool = static_cast<__nv_bfloat16*>(pools.p[blockIdx.y]) +
                         (size_t)(col / per_head) * a.block_size * a.head_dim + (col % per_head) * 8;
-  for (int j0 = 1; j0 <= acc; j0 += KEEP_BATCH) {
+  int first = 1;   // the first nodes of the path are often in their place already
+  while (first <= acc && s_src[first] == s_dst[first]) ++first;
+  for (int j0 = first; j0 <= acc; j0 += KEEP_BATCH) {
     uint4 v[KEEP_BATCH];
 #pragma unroll
     for (int k = 0; k < KEEP_BATCH; ++k)
