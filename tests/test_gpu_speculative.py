@@ -680,6 +680,23 @@ def test_keep_path(layers, hkv, bs, hd, stacked):
         assert torch.equal(want, d.cpu())
 
 
+@pytest.mark.parametrize("bs", [1, 4, 16])
+def test_keep_path_partly_in_place(bs):
+    """Paths whose first nodes, or all of them, stay where they are."""
+    paths = [[0, 1, 2, 3, 4, 5], [0, 1, 2, 3, 4, 6], [0, 1, 2, 5, 7, -1], [0, 1, -1, -1, -1, -1],
+             [0, 2, -1, -1, -1, -1]]
+    took, q_lens, ctx = [5, 5, 4, 1, 1], [8] * 5, [8, 21, 33, 40, 11]
+    need = [-(-c // bs) for c in ctx]
+    ids = torch.randperm(sum(need), generator=torch.Generator().manual_seed(bs)).tolist()
+    tables = [ids[sum(need[:i]):sum(need[:i + 1])] for i in range(5)]
+    host = random_pools(3, len(ids), 2, bs, 64)
+    dev = [p.to(DEV) for p in host]
+    ops.keep_kv_path(dev, block_tables=i32([t + [-1] * (max(need) - len(t)) for t in tables]), q_len=i32(q_lens),
+                     ctx_len=i32(ctx), path=i32(paths), n_accepted=i32(took))
+    for want, d in zip(R.keep_path(host, tables, q_lens, ctx, paths, took), dev):
+        assert torch.equal(want, d.cpu())
+
+
 def test_keep_path_long_paths():
     """More accepted nodes than one batch of loads, chains shifted by one."""
     host = random_pools(2, 40, 2, 16, 64)
