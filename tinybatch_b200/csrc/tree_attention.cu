@@ -164,27 +164,30 @@ static int tree_simple_launch(const TreeAttnArgs& t, cudaStream_t st) {
 //              contiguous), landing as [8-token group][half][8][128 B] with the
 //              128-byte swizzle: K is a K-major operand and V an MN-major one.  Four
 //              lanes issue a tile's boxes.  Other block sizes: 16-byte cp.async
-//              pieces into the same layout, every key looking up its block (half as
-//              long again).  K and V have rings of their own: a K stage is free once
-//              its S is done, before the V that came with it
+//              pieces into the same layout, every key looking up its block (1.25 to 2
+//              times as long: blocks of 8 take 10 / 88 / 69 / 323 us where blocks of
+//              16 take 8 / 58 / 48 / 161 on the cases below, the lone one first).  K
+//              and V have rings of their own: a K stage is free once its S is done,
+//              before the V that came with it
 //   warp 5     MMA issue.  P (bf16) has two buffers of its own in TMEM, so S of the
 //              next tile follows as soon as the softmax has S in registers and is
 //              there when it has written P
 // O is accumulated in TMEM; a row's exponent reference moves only when its
 // maximum has grown by more than TT_RESCALE (log2 units), as in the prefill kernel.
 // Two CTAs an SM: one's chain S -> softmax -> P V, its start and its end hide
-// behind the other's loads.  Of mma.sync, which reaches a few hundred TFLOP/s, the rows
-// of a tree (nodes x heads of the group, up to 512 here) would ask more than HBM does.
+// behind the other's loads.
 //
 // Measured on a B200 (CUDA graph, inputs rotated through more than the L2): 32
 // chains of 6 drafts over 500-4000 tokens (40/8 heads of 128) 57.5 us, 5.3 TB/s or
 // 0.81 of the measured copy bandwidth; 16 trees of 25 over 300-6000 tokens 48.4 us,
-// 0.61 of it (what is missing: the splits' exchange over the cluster, ~3 us a CTA, and
-// the tail of the ragged batch); 4 trees of 64 over 12-20 thousand tokens, 512 rows
-// a kv head, 154 us, 880 TFLOP/s or 0.54 of the measured bf16 peak: there the
-// softmax's chain of dependent instructions bounds it (tensor pipe 52% busy,
-// exponentials 49%).  A lone short request takes 7.7 us: launch, lengths, block ids, K,
-// S, softmax, P V and the store one after another.
+// 0.61 of it (what is missing: ~2.5 us before a CTA's first tile, 4-5 us of merge over
+// the cluster with the wait for its members, the tail of the ragged batch); 4 trees of
+// 64 over 12-20 thousand tokens, 512 rows a kv head, 154-162 us from board to board,
+// 880-835 TFLOP/s or 0.54-0.51 of the measured bf16 peak: there the softmax's chain of
+// dependent instructions bounds it (tensor pipe 52% busy, exponentials 49%).  A lone
+// short request takes 7.7-8.0 us: launch, lengths, block ids, K, S, softmax, P V and
+// the store one after another.  At the 128 registers a thread 11 words spill at
+// head_dim 128 (8 at 64); with more registers a CTA waits for an empty SM.
 // Tried and dropped: 16-byte cp.async for all loads (one warp issues 9 B a cycle: 94
 // instead of 64 us for the trees), two threads a row (the exchange of maxima costs what
 // the shorter softmax saves), K and V boxes issued together (K waits for V's stage).

@@ -27,12 +27,13 @@
 // move with the summation order in 32.
 //
 // What bounds them (B200, CUDA graph, vocabulary 152064).  Greedy: launch and two
-// dependent loads, 2.2 us for one sequence, 3.3 us for 128.  Sampled: ~1.9 us of
-// dependent loads (rows, tree, the drafts' probabilities) and ~1.4 us of walk, then one
-// pass over the last node's rows and ~1.3 us of search.  One sequence, outright
-// drafts 8.8 us; 64 chains 26.5 us, of them ~15 in the pass (78 MB, the floor of the
-// call is 11.9 us); 8 trees of 40 nodes 23 us: up to eight dependent passes of
-// ~1.6 us (each Z decides the next sibling's test) where the floor counts one.
+// dependent loads, 2.4 us for one sequence, 3.3 us for 128.  Sampled: steps that wait
+// for one another.  One sequence, outright drafts 8.8 us; stamps of an instrumented
+// build: loads of rows, tree and probabilities 2.1 us, walk 1.7, pass over the last
+// node's rows 1.9, sums over the cluster 1.4, search 2.4.  64 chains 26.5 us, of them
+// ~14 in the pass (78 MB, the floor of the call is 11.9 us).  8 trees of 40 nodes
+// 23.3 us: the slowest walk takes 13, as each Z is a pass that decides the next
+// sibling's test; the floor counts one pass.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
