@@ -558,6 +558,33 @@ def test_verify_refuses_arguments():
     ops.verify_drafts(ids[:0], ids[:0], ids[:0], ids[:0], p[:0], u[:0], took[:0], path[:0], nxt[:0])
 
 
+def test_verify_without_any_draft_distribution():
+    """draft_probs without rows: what None says, and a row that names one is reported."""
+    p, u = torch.full((2, 3), 1 / 3, device=DEV), torch.tensor([0.5, 0.2], device=DEV)
+    base = (i32([0, 1]), i32([-1, 0]), i32([0]), i32([2]), p, u)
+    want = outputs(1, 2)
+    ops.verify_drafts(*base, *want)
+    for rows in ([-1, -1], [0, -1]):
+        got = outputs(1, 2)
+        ops.verify_drafts(*base, *got, draft_probs=p[:0], draft_rows=i32(rows))
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+        assert _native.status(clear=True) == (BAD_INDEX if rows[0] == 0 else 0)
+
+
+def test_verify_of_sequences_without_any_row():
+    """A padded batch that holds no tree: nothing accepted, nothing chosen."""
+    none, zeros = torch.empty(0, dtype=torch.int32, device=DEV), i32([0, 0, 0])
+    probs, u = torch.empty(0, 50, device=DEV), torch.empty(0, device=DEV)
+    for call in (lambda *o: ops.verify_drafts_greedy(none, none, zeros, zeros, none, *o),
+                 lambda *o: ops.verify_drafts(none, none, zeros, zeros, probs, u, *o),
+                 lambda *o: ops.verify_drafts(none, none, zeros, zeros, probs, u, *o, draft_probs=probs,
+                                              draft_rows=none)):
+        took, path, nxt = outputs(3, 4)
+        call(took, path, nxt)
+        assert (took.tolist(), path.tolist(), nxt.tolist()) == ([0] * 3, [[-1] * 4] * 3, [-1] * 3)
+
+
 def test_verify_captured_and_replayed():
     g = torch.Generator().manual_seed(1)
     p = distributions(g, 12, 5000).to(DEV)

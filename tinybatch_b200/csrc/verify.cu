@@ -590,9 +590,11 @@ static int check_tree(const TreeArgs& t, int max_q) {
   if (t.n_seqs < 0 || t.n_rows < 0 || t.path_w <= 0 || t.path_ld < t.path_w)
     return arg_err("n_seqs / n_rows / path width");
   if (max_q > VF_NODES) return arg_err("a draft tree has at most 256 nodes");
-  if (t.n_seqs > 0 && (t.ids == nullptr || t.parents == nullptr || t.q_start == nullptr ||
-                       t.q_len == nullptr || t.n_accepted == nullptr || t.path == nullptr ||
-                       t.next_ids == nullptr))
+  if (t.n_seqs > 0 && (t.q_start == nullptr || t.q_len == nullptr || t.n_accepted == nullptr ||
+                       t.path == nullptr || t.next_ids == nullptr))
+    return arg_err("null pointer");
+  // (a padded batch may have no rows at all)
+  if (t.n_seqs > 0 && t.n_rows > 0 && (t.ids == nullptr || t.parents == nullptr))
     return arg_err("null pointer");
   return TB_OK;
 }
@@ -600,7 +602,7 @@ static int check_tree(const TreeArgs& t, int max_q) {
 int verify_greedy_launch(const TreeArgs& t, const int* target_ids, int max_q, cudaStream_t st) {
   if (int rc = check_tree(t, max_q)) return rc;
   if (t.n_seqs == 0) return TB_OK;
-  if (target_ids == nullptr) return arg_err("null pointer");
+  if (t.n_rows > 0 && target_ids == nullptr) return arg_err("null pointer");
   return launch_pdl(verify_greedy_kernel, dim3((t.n_seqs + VG_WARPS - 1) / VG_WARPS),
                     dim3(VG_WARPS * 32), 0, st, 1, "greedy verification launch", t, target_ids);
 }
@@ -608,9 +610,10 @@ int verify_greedy_launch(const TreeArgs& t, const int* target_ids, int max_q, cu
 int verify_launch(const VerifyArgs& a, int max_q, cudaStream_t st) {
   if (int rc = check_tree(a.t, max_q)) return rc;
   if (a.t.n_seqs == 0) return TB_OK;
-  if (a.vocab <= 0 || a.vocab > (1 << 28) || a.ld_p < a.vocab || a.probs == nullptr || a.uniforms == nullptr)
+  if (a.vocab <= 0 || a.vocab > (1 << 28) || a.ld_p < a.vocab ||
+      (a.t.n_rows > 0 && (a.probs == nullptr || a.uniforms == nullptr)))
     return arg_err("probs / vocab / uniforms");
-  if ((a.draft_probs == nullptr) != (a.draft_rows == nullptr))
+  if (a.t.n_rows > 0 && (a.draft_probs == nullptr) != (a.draft_rows == nullptr))
     return arg_err("draft_probs and draft_rows go together");
   if (a.draft_probs != nullptr && (a.ld_d < a.vocab || a.n_draft_rows < 0))
     return arg_err("draft_probs shape");

@@ -295,7 +295,8 @@ def verify_drafts(ids, parents, q_start, q_len, probs, uniforms, n_accepted, pat
         dp, ldd, cols = _mat("draft_probs", draft_probs, _F32, None, dev)
         if cols != vocab:
             raise ValueError(f"draft_probs: expected {vocab} columns, got {cols}")
-        draft = (dp, ldd, len(draft_probs), _vec("draft_rows", draft_rows, _I32, rows, dev))
+        # (without any distribution there is no address, and no row may name one)
+        draft = (dp or pp, ldd, len(draft_probs), _vec("draft_rows", draft_rows, _I32, rows, dev))
     _run_on(dev, "tb_verify_drafts", lib.tb_verify_drafts, *tree, n, rows[0], max_q, pp, ldp, vocab,
             *draft, up, *outs)
 
