@@ -14,6 +14,7 @@ from tinybatch_b200 import _native as N
 from tinybatch_b200 import ops
 from tinybatch_b200.block_manager import BlockManager, OutOfBlocks
 from tinybatch_b200.kv_cache import PagedKVCache
+from tinybatch_b200.model import Qwen2Paged
 from tinybatch_b200.runtime import StepMeta, tree_masks
 
 P = 256     # stands for an aligned pointer that is never followed
@@ -159,6 +160,18 @@ def test_step_metadata_of_trees():
         StepMeta([1, 2], [16, 17], [(0, 2)], [[3]], [18], 16, 2, "cpu", pinned=False, trees=mask[:2])
     with pytest.raises(ValueError):
         StepMeta([1, 2], [0, 1], [(0, 2)], [[3]], [2], 16, 2, "cpu", pinned=False, trees=mask[:1])
+
+
+@pytest.mark.parametrize("ids,parents,tables,ctx,needle", [
+    ([], [], [], [], "at least one tree"), ([1, 2], [[-1, 0, 0]], [[0]], [10], "3 nodes, 2 token ids"),
+    ([1, 2, 3, 4], [[-1, 0, 0]], [[0]], [10], "3 nodes, 4 token ids"), ([1], [[-1]], [], [10], "per tree"),
+    ([1], [[-1]], [[0]], [10, 11], "per tree"), ([1, 2], [[-1, 0]], [[0]], [1], "context holds"),
+    ([1], [[-1], []], [[0], [1]], [10, 5], "has a root")])
+def test_forward_tree_argument_errors(ids, parents, tables, ctx, needle):
+    class OneRank:
+        world = 1
+    with pytest.raises(ValueError, match=needle):
+        Qwen2Paged.forward_tree(OneRank(), ids, parents, tables, ctx, None)
 
 
 def test_fork_and_trim_tables():

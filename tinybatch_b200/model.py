@@ -105,8 +105,10 @@ class Qwen2Paged:
             raise RuntimeError("forward_tree runs on one rank")
         parents = [_to_list(p) for p in parents]
         ctx = _to_list(context_lens)
-        if len(ctx) != len(parents):
-            raise ValueError("one context length per tree")
+        if not parents:
+            raise ValueError("forward_tree needs at least one tree")
+        if len(ctx) != len(parents) or len(block_tables) != len(parents):
+            raise ValueError("one context length and one block table per tree")
         mask, depth = tree_masks(parents)
         slices, pos, r0 = [], [], 0
         for par, c in zip(parents, ctx):
@@ -115,7 +117,10 @@ class Qwen2Paged:
             slices.append((r0, r0 + len(par)))
             pos += [c - len(par) + int(d) for d in depth[r0:r0 + len(par)]]
             r0 += len(par)
-        md = StepMeta(_to_list(token_ids), pos, slices, [list(t) for t in block_tables], ctx,
+        ids = _to_list(token_ids)
+        if len(ids) != r0:
+            raise ValueError(f"{r0} nodes, {len(ids)} token ids")
+        md = StepMeta(ids, pos, slices, [list(t) for t in block_tables], ctx,
                       kv_cache.block_size, self.cfg.n_heads // self.cfg.n_kv_heads, self.device,
                       all_logits=True, trees=mask)
         logits = self.dm.forward(md, kv_cache.pools, sample=sample)
