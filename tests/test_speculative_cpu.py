@@ -174,6 +174,15 @@ def test_forward_tree_argument_errors(ids, parents, tables, ctx, needle):
         Qwen2Paged.forward_tree(OneRank(), ids, parents, tables, ctx, None)
 
 
+def test_forward_tree_refuses_blocks_outside_the_pool():
+    class OneRank:
+        world = 1
+    cache = PagedKVCache(1, 4, 16, 1, 64, device="cpu")
+    for tables in ([[0, 4], [1]], [[0, 1], [2**30]]):
+        with pytest.raises(IndexError, match="out of range"):
+            Qwen2Paged.forward_tree(OneRank(), [5, 6], [[-1], [-1]], tables, [20, 3], cache)
+
+
 def test_fork_and_trim_tables():
     bm = BlockManager(8, 4, False)
     table, _ = bm.allocate_prompt(list(range(10)))                # 2 full blocks and half a third

@@ -120,7 +120,10 @@ class Qwen2Paged:
         ids = _to_list(token_ids)
         if len(ids) != r0:
             raise ValueError(f"{r0} nodes, {len(ids)} token ids")
-        md = StepMeta(ids, pos, slices, [list(t) for t in block_tables], ctx,
+        tables = [_to_list(t) for t in block_tables]
+        if any(b >= kv_cache.num_blocks for t in tables for b in t):
+            raise IndexError("block id out of range")    # its K/V would land behind the pool
+        md = StepMeta(ids, pos, slices, tables, ctx,
                       kv_cache.block_size, self.cfg.n_heads // self.cfg.n_kv_heads, self.device,
                       all_logits=True, trees=mask)
         logits = self.dm.forward(md, kv_cache.pools, sample=sample)
