@@ -113,6 +113,16 @@ def test_cpu_tensors_are_refused():
         ops.verify_drafts_greedy(t, t, t, t, t, t, t[None], t)
 
 
+def test_row_pitches_of_more_than_31_bits_are_refused():
+    """They would wrap in the C entries' arguments (nothing is allocated: meta tensors)."""
+    def rows(pitch):
+        return torch.empty_strided((2, 4), (pitch, 1), dtype=torch.int32, device="meta")
+    assert ops._mat("path", rows(2**31 - 1), torch.int32, 2, -1)[1:] == (2**31 - 1, 4)
+    for pitch in (2**31, 2**32 + 8):
+        with pytest.raises(ValueError, match="path"):
+            ops._mat("path", rows(pitch), torch.int32, 2, -1)
+
+
 def test_copy_blocks_checks_its_pairs_on_the_host():
     cache = PagedKVCache(1, 4, 16, 1, 64, device="cpu")
     cache.copy_blocks([])

@@ -185,12 +185,14 @@ def _vec(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev: int)
 
 
 def _mat(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int | None, dev: int):
-    """(pointer, row pitch, columns) of a 2-d argument with contiguous rows."""
+    """(pointer, row pitch, columns) of a 2-d argument with contiguous rows; the C
+    entries take 32-bit pitches."""
     shape = t.shape
     if t.dtype is dtype and len(shape) == 2 and t.get_device() == dev:
         n, cols = shape
         pitch, step = t.stride()
-        if (rows is None or n == rows) and (step == 1 or cols <= 1):
+        if (rows is None or n == rows) and (step == 1 or cols <= 1) and (
+                pitch < 0x80000000 or n <= 1):
             return t.data_ptr(), (pitch if n > 1 else cols), cols
     _refuse(name, t, f"a 2-d {dtype} tensor of {'any' if rows is None else rows} contiguous rows",
             dev)
