@@ -238,6 +238,52 @@ def test_fork_keeps_prefix_cached_blocks_cached():
     assert bm.num_free() == 4 and bm.allocate_prompt(list(range(8)))[1] == 8
 
 
+def test_trimmed_drafts_leave_the_prefix_cache():
+    """Drafts that append_slot published are not found any more once they are
+    trimmed: neither in the block that keeps accepted tokens (later tokens
+    overwrite it) nor in a released one."""
+    prompt, drafts = [1, 2, 3, 4, 5, 6], [70, 80, 90, 91, 92, 93, 94]
+    for kept, cached in ((6, 4), (7, 4), (8, 8), (9, 8), (12, 12)):
+        bm = BlockManager(8, 4, True)
+        table, _ = bm.allocate_prompt(prompt)
+        tokens = list(prompt)
+        for t in drafts:
+            bm.append_slot(table, tokens)
+            tokens.append(t)
+        assert len(table) == 4 and sum(b.prefix_hash is not None for b in bm.blocks) == 3
+        bm.trim_table(table, kept)
+        assert bm.num_free() == 8 - len(table) and not bm.evictable
+        assert all(bm.blocks[b].prefix_hash in bm.cache for b in bm.cache.values())
+        other, hit = bm.allocate_prompt(tokens)
+        assert hit == cached and other[:cached // 4] == table[:cached // 4]
+        assert not set(other[cached // 4:]) & set(table)
+        # the accepted continuation is published under its own tokens
+        bm.free_table(other)
+        tokens = tokens[:kept] + [500 + i for i in range(9)]
+        for n in range(kept, len(tokens)):
+            bm.append_slot(table, tokens[:n])
+        full = (len(tokens) - 1) // 4        # append_slot publishes a block when the next one opens
+        assert bm.allocate_prompt(tokens)[1] == 4 * full
+
+
+def test_trim_keeps_what_others_share():
+    """Shared blocks stay published for their other tables; a trim that would leave the
+    next token to a shared block changes nothing."""
+    bm = BlockManager(8, 4, True)
+    table, _ = bm.allocate_prompt(list(range(12)))
+    other, hit = bm.allocate_prompt(list(range(12)))
+    assert hit == 12 and other == table
+    for tokens in (6, 11, -1):
+        with pytest.raises(ValueError):
+            bm.trim_table(other, tokens)
+        assert other == table and [bm.blocks[b].ref_count for b in table] == [2, 2, 2]
+    bm.trim_table(other, 4)
+    assert other == table[:1] and [bm.blocks[b].ref_count for b in table] == [2, 1, 1]
+    assert bm.allocate_prompt(list(range(12)))[1] == 12
+    with pytest.raises(ValueError, match="negative"):
+        bm.trim_table(other, -100)
+
+
 def test_oracle_follows_the_target_exactly():
     """The restatement's acceptance and residual, integrated over the draft and the
     test's uniform number on a grid, give the target's distribution: two

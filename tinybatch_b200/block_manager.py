@@ -185,7 +185,29 @@ class BlockManager:
 
     def trim_table(self, table: list[int], num_tokens: int) -> None:
         """Release the blocks of ``table`` behind its first ``num_tokens`` tokens
-        (those that held rejected drafts), last first."""
-        keep = self.blocks_needed(num_tokens)
+        (those that held rejected drafts), last first.  A block that reaches
+        past ``num_tokens`` and belongs to this table alone leaves the prefix
+        cache: its hash names drafts that later tokens overwrite.  Raises
+        ValueError, and changes nothing, when ``num_tokens`` ends inside a
+        block that other tables share (``fork_table`` gives the sequence a
+        copy of its own)."""
+        if num_tokens < 0:
+            raise ValueError("num_tokens is negative")
+        full, tail = divmod(num_tokens, self.block_size)
+        if tail and full < len(table):
+            last = self.blocks[table[full]]
+            if last.ref_count > 1:
+                raise ValueError("the last kept block is shared")
+            self._unpublish(last)
+            last.token_ids = last.token_ids[:tail]
+        keep = full + (tail > 0)
         while len(table) > keep:
-            self.free_table([table.pop()])
+            blk = self.blocks[table.pop()]
+            if blk.ref_count == 1:
+                self._unpublish(blk)
+            self.free_table([blk.block_id])
+
+    def _unpublish(self, blk: Block) -> None:
+        if blk.prefix_hash is not None:
+            self.cache.pop(blk.prefix_hash, None)
+            blk.prefix_hash = None
