@@ -266,6 +266,64 @@ def test_trimmed_drafts_leave_the_prefix_cache():
         assert bm.allocate_prompt(tokens)[1] == 4 * full
 
 
+def test_room_for_drafts_is_published_once_accepted():
+    """reserve / trim_table / publish over several steps: what other prompts find is
+    always a prefix of accepted tokens, and every full block of them."""
+    bm = BlockManager(32, 4, True)
+    tokens = [1, 2, 3, 4, 5, 6]                       # the last one's K/V are written by the next forward
+    table, _ = bm.allocate_prompt(tokens[:5])
+    for step, took in enumerate((0, 3, 1, 0, 4, 4, 2)):
+        drafts = [1000 * step + j for j in range(1, 6)]
+        bm.reserve(table, len(tokens) + len(drafts))
+        assert len(table) == bm.blocks_needed(len(tokens) + len(drafts))
+        other, hit = bm.allocate_prompt(tokens + drafts)
+        assert hit == (len(tokens) - 1) // 4 * 4      # no draft is found while it may be rejected
+        assert not set(other[hit // 4:]) & set(table)
+        bm.free_table(other)
+        for bid in other[hit // 4:]:                  # (forget what this look published)
+            if bm.blocks[bid].prefix_hash is not None:
+                bm.evictable.pop(bid)
+                bm._unpublish(bm.blocks[bid])
+                bm.free_ids.append(bid)
+        before = len(tokens)
+        tokens += drafts[:took] + [1000 * step + 9]
+        bm.trim_table(table, len(tokens) - 1)
+        assert len(table) == bm.blocks_needed(len(tokens) - 1)
+        bm.publish(table, tokens[:-1], before - 1)
+        assert bm.blocks[table[0]].ref_count == 1
+    other, hit = bm.allocate_prompt(tokens)
+    assert hit == (len(tokens) - 1) // 4 * 4 and other[:hit // 4] == table[:hit // 4]
+    with pytest.raises(ValueError):
+        bm.publish(table, tokens + [0] * 4)
+    # the next token by append_slot, in the room that trim_table left
+    fresh = BlockManager(8, 4, True)
+    table, _ = fresh.allocate_prompt([1, 2, 3])
+    fresh.reserve(table, 9)
+    fresh.trim_table(table, 4)
+    assert fresh.append_slot(table, [1, 2, 3, 4]) and len(table) == 2
+    assert fresh.allocate_prompt([1, 2, 3, 4])[1] == 4
+
+
+def test_reserve_takes_all_blocks_or_none():
+    bm = BlockManager(4, 4, True)
+    old, _ = bm.allocate_prompt(list(range(8)))
+    bm.free_table(old)                                # two cached blocks, evictable
+    table, _ = bm.allocate_prompt([50])
+    with pytest.raises(OutOfBlocks):
+        bm.reserve(table, 17)
+    assert len(table) == 1 and bm.num_free() == 3 and len(bm.cache) == 2
+    bm.reserve(table, 1)
+    bm.reserve(table, 0)
+    assert len(table) == 1
+    bm.reserve(table, 16)
+    assert len(table) == len(set(table)) == 4 and bm.num_free() == 0 and not bm.cache
+    bm.trim_table(table, 0)
+    off = BlockManager(2, 4, False)
+    table, _ = off.allocate_prompt([1, 2, 3, 4])
+    off.publish(table, [1, 2, 3, 4])
+    assert not off.cache
+
+
 def test_trim_keeps_what_others_share():
     """Shared blocks stay published for their other tables; a trim that would leave the
     next token to a shared block changes nothing."""

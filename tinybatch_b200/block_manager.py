@@ -183,6 +183,26 @@ class BlockManager:
             self.blocks[bid].ref_count += 1
         return new, copies
 
+    def reserve(self, table: list[int], num_tokens: int) -> None:
+        """Make room for ``num_tokens`` tokens in ``table``, drafts among them:
+        fresh blocks, none of them published (``append_slot`` publishes the
+        block before a new one, drafts or not).  Changes nothing when the pool
+        cannot supply them all."""
+        need = self.blocks_needed(num_tokens) - len(table)
+        if need > self.num_free():
+            raise OutOfBlocks(f"{need} blocks needed, {self.num_free()} free")
+        table += [self._own(self._fresh_block(), []).block_id for _ in range(need)]
+
+    def publish(self, table: list[int], token_ids: list[int], start: int = 0) -> None:
+        """Put the full blocks of ``table`` into the prefix cache under
+        ``token_ids``, the accepted tokens whose K/V they hold; ``start``: how
+        many of these an earlier call covered."""
+        if len(token_ids) > len(table) * self.block_size:
+            raise ValueError("the table does not hold that many tokens")
+        if self.enable_prefix_caching:
+            for idx in range(start // self.block_size, len(token_ids) // self.block_size):
+                self._publish(table, idx, token_ids)
+
     def trim_table(self, table: list[int], num_tokens: int) -> None:
         """Release the blocks of ``table`` behind its first ``num_tokens`` tokens
         (those that held rejected drafts), last first.  A block that reaches
