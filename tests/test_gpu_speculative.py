@@ -301,6 +301,22 @@ def test_tree_attention_bad_metadata_is_refused(hd, bs):
     assert torch.equal(out[:8], good[:8])
 
 
+@pytest.mark.parametrize("hq,hkv,hd,bs", [(4, 2, 64, 16), (10, 2, 128, 8), (4, 2, 16, 4)])
+def test_tree_attention_lengths_whose_difference_wraps_are_refused(hq, hkv, hd, bs):
+    """ctx_len near -2^31: ctx_len - q_len leaves 32 bits and must not pass for a long prefix."""
+    c = Case(hq, hkv, hd, bs, [4, 4, 4], [30, 30, 30], seed=15)
+    d = c.device()
+    good = c.run(d)
+    rest = [0, 1, 2, 3, 8, 9, 10, 11]
+    for value in (-2**31, -2**31 + 1, -2**31 + 3, -2**31 + 4):
+        bad = dict(d, ctx=d["ctx"].clone())
+        bad["ctx"][1] = value
+        out = c.run(bad)
+        torch.cuda.synchronize()
+        assert _native.status(clear=True) == BAD_INDEX
+        assert torch.equal(out[rest], good[rest]) and bool(out[4:8].isnan().all())
+
+
 def test_tree_attention_refuses_arguments():
     c = Case(4, 2, 64, 16, [4], [30], seed=16)
     d = c.device()
