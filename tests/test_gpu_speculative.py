@@ -772,6 +772,19 @@ def test_keep_path_bad_sequences_move_nothing(change):
         assert torch.equal(want, d.cpu())
 
 
+@pytest.mark.parametrize("ctx", [-2**31, -2**31 + 3, -2**31 + 5, 5])
+def test_keep_path_lengths_whose_difference_wraps_move_nothing(ctx):
+    """ctx_len - q_len must not pass for a position after leaving 32 bits."""
+    host = random_pools(2, 8, 2, 16, 64)
+    dev = [p.to(DEV) for p in host]
+    ops.keep_kv_path(dev, block_tables=i32([[4, 2], [5, 6]]), q_len=i32([6, 5]), ctx_len=i32([ctx, 18]),
+                     path=i32([[0, 1, 3, 5], [0, 2, 4, -1]]), n_accepted=i32([3, 2]))
+    torch.cuda.synchronize()
+    assert _native.status(clear=True) == BAD_INDEX
+    for want, d in zip(R.keep_path(host, [[5, 6]], [5], [18], [[0, 2, 4, -1]], [2]), dev):
+        assert torch.equal(want, d.cpu())
+
+
 # ------------------------------------------------------------------ together
 
 

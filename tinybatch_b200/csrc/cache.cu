@@ -107,8 +107,8 @@ __global__ void __launch_bounds__(KEEP_THREADS)
   if (acc == 0) return;
   const int* path = a.path + (size_t)seq * a.path_ld;
   const int* table = a.block_tables + (size_t)seq * a.bt_ld;
-  const int base = ctx - ql;
-  int bad = acc < 0 || acc >= a.path_w || acc >= ql || ql > KEEP_MAX || base < 0 ||
+  const int base = ctx - ql;   // (used only where ctx >= ql: elsewhere it may wrap)
+  int bad = acc < 0 || acc >= a.path_w || acc >= ql || ql > KEEP_MAX || ctx < ql ||
             (int)(((long long)ctx + a.block_size - 1) / a.block_size) > a.bt_w;
   if (!bad) {
     const size_t token = a.head_dim;
