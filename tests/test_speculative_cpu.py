@@ -193,6 +193,27 @@ def test_forward_tree_refuses_blocks_outside_the_pool():
             Qwen2Paged.forward_tree(OneRank(), [5, 6], [[-1], [-1]], tables, [20, 3], cache)
 
 
+def test_forward_tree_refuses_negative_blocks_inside_the_context():
+    """A slot of a negative block wraps to another sequence's (-2^28 * 16 is slot 0 in 32
+    bits); -1 may pad the table behind the context only."""
+    class OneRank:
+        world, device = 1, "cpu"
+
+        class cfg:
+            n_heads, n_kv_heads = 2, 1
+
+        class dm:
+            @staticmethod
+            def forward(md, pools, sample):
+                return None
+    cache = PagedKVCache(1, 4, 16, 1, 64, device="cpu")
+    for table in ([0, -1], [-1, 0], [-2**28, 0], [0, -2**28]):
+        with pytest.raises(IndexError, match="out of range"):
+            Qwen2Paged.forward_tree(OneRank(), [5], [[-1]], [table], [17], cache)
+    md, _ = Qwen2Paged.forward_tree(OneRank(), [5, 6], [[-1], [-1]], [[3, -1], [0, 2]], [16, 17], cache)
+    assert md.slots.tolist() == [63, 32] and md.tree_bt.tolist() == [[3, -1], [0, 2]]
+
+
 def test_fork_and_trim_tables():
     bm = BlockManager(8, 4, False)
     table, _ = bm.allocate_prompt(list(range(10)))                # 2 full blocks and half a third

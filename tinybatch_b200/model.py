@@ -121,10 +121,11 @@ class Qwen2Paged:
         if len(ids) != r0:
             raise ValueError(f"{r0} nodes, {len(ids)} token ids")
         tables = [_to_list(t) for t in block_tables]
-        if any(b >= kv_cache.num_blocks for t in tables for b in t):
-            raise IndexError("block id out of range")    # its K/V would land behind the pool
-        md = StepMeta(ids, pos, slices, tables, ctx,
-                      kv_cache.block_size, self.cfg.n_heads // self.cfg.n_kv_heads, self.device,
+        bs = kv_cache.block_size
+        if any(b >= kv_cache.num_blocks for t in tables for b in t) or any(
+                b < 0 for t, c in zip(tables, ctx) for b in t[:-(-c // bs)]):   # -1 pads behind it
+            raise IndexError("block id out of range")    # its K/V would land outside the pool
+        md = StepMeta(ids, pos, slices, tables, ctx, bs, self.cfg.n_heads // self.cfg.n_kv_heads, self.device,
                       all_logits=True, trees=mask)
         logits = self.dm.forward(md, kv_cache.pools, sample=sample)
         return md, (self.dm.next_ids[:md.T] if sample else logits)
