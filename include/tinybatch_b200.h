@@ -317,8 +317,9 @@ int tb_argmax(const float* logits, int ld, int M, int N, int* out, void* stream)
  * 0 = bt_w * block_size / n_seqs times that).  No scratch: the blocks that
  * share a context form a cluster and merge through shared memory.
  * A sequence whose rows leave the batch, whose q_len exceeds max_q or the
- * mask, or whose context its block-table row cannot hold, and block ids out
- * of range set TB_STATUS_BAD_INDEX. */
+ * mask, whose context its block-table row cannot hold, or whose context lies
+ * in a block out of range sets TB_STATUS_BAD_INDEX; its rows of out are left
+ * as they were. */
 int tb_paged_attention_tree(const void* q, int ld_q, void* out, int ld_out, int n_rows,
                             const void* kv_pool, int num_blocks, int n_q_heads,
                             int n_kv_heads, int head_dim, int block_size,

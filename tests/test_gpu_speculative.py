@@ -317,6 +317,28 @@ def test_tree_attention_lengths_whose_difference_wraps_are_refused(hq, hkv, hd, 
         assert torch.equal(out[rest], good[rest]) and bool(out[4:8].isnan().all())
 
 
+@pytest.mark.parametrize("hq,hkv,hd,bs", [(10, 2, 128, 16), (14, 2, 64, 16), (10, 2, 128, 8), (4, 2, 16, 4)])
+@pytest.mark.parametrize("at", [0, -1])
+def test_tree_attention_leaves_sequences_with_bad_blocks_out(hq, hkv, hd, bs, at):
+    """A block id out of range, the first of a context or the last (nodes that few rows
+    see): every row of the sequence stays as it was, whether one CTA or
+    several share the context; the others' bits do not change."""
+    c = Case(hq, hkv, hd, bs, [30, 30, 4], [600, 9, 40], seed=17)
+    d = c.device()
+    for split in (dict(max_ctx=630, ctx_total=630 + 39 + 44), dict(max_ctx=1, ctx_total=1)):
+        good = c.run(d, **split)
+        for seq in range(3):
+            for value in (c.pool.shape[0], -1, 2**31 - 1, -2**31):
+                bad = dict(d, bt=d["bt"].clone())
+                bad["bt"][seq, at % len(c.tables[seq])] = value
+                out = c.run(bad, **split)
+                torch.cuda.synchronize()
+                assert _native.status(clear=True) == BAD_INDEX
+                lost = range(c.q_start[seq], c.q_start[seq] + c.q_lens[seq])
+                rest = [i for i in range(64) if i not in lost]
+                assert torch.equal(out[rest], good[rest]) and bool(out[list(lost)].isnan().all())
+
+
 def test_tree_attention_refuses_arguments():
     c = Case(4, 2, 64, 16, [4], [30], seed=16)
     d = c.device()

@@ -85,15 +85,16 @@ __global__ void __launch_bounds__(TS_WARPS * 32) tree_attn_simple_kernel(const T
 #pragma unroll
   for (int k = 0; k < CPL; ++k) o[k] = 0.f;
   float m = -INFINITY, l = 0.f;
+  bool lost = false;      // a block id out of range: the sequence is left out
   for (int p0 = 0; p0 < s.ctx; p0 += 32) {
     const int p = p0 + lane;
     bool seen = p < s.ctx;
     if (p >= s.base && seen) seen = (mask[(p - s.base) >> 6] >> ((p - s.base) & 63)) & 1;
     size_t off = 0;
-    if (seen) {
+    if (p < s.ctx) {
       const int blk = table[p / a.block_size];
       if (blk < 0 || blk >= a.num_blocks) {
-        set_status(ERR_BAD_INDEX);
+        lost = true;
         seen = false;
       } else {
         off = ((size_t)blk * 2 * a.n_kv_heads + kvh) * head + (size_t)(p % a.block_size) * HD;
@@ -136,6 +137,10 @@ __global__ void __launch_bounds__(TS_WARPS * 32) tree_attn_simple_kernel(const T
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (__any_sync(0xffffffffu, lost)) {
+    if (lane == 0) set_status(ERR_BAD_INDEX);
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int k = 0; k < CPL; ++k)
@@ -207,6 +212,9 @@ constexpr int TT_KEYS = 64;
 constexpr int TT_THREADS = 192;
 constexpr float TT_RESCALE = 8.f;
 constexpr int TT_MAX_SPLITS = 8;
+// What a CTA found; the members of a cluster merge theirs.
+constexpr int TT_NONFINITE = 1;   // a draft's V has non-finite elements
+constexpr int TT_LOST = 2;        // a block id is out of range: the sequence is left out
 
 // Shared memory of a CTA: Q (only the warps' rows that exist: the MMA reads 128
 // rows whatever they hold, the others' results are never looked at), then as many
@@ -270,8 +278,8 @@ __device__ __forceinline__ uint64_t sw128_k_desc(uint32_t smem_addr, uint32_t sb
 __device__ __forceinline__ void st_cluster_f2(uint32_t addr, float x, float y) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(addr), "f"(x), "f"(y) : "memory");
 }
-__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t x) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
+__device__ __forceinline__ void red_cluster_or(uint32_t addr, uint32_t x) {
+  asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
 }
 
 // True in one lane of the (converged) warp, the same one every time.
@@ -401,7 +409,7 @@ __global__ void __launch_bounds__(256, 2)
   uint64_t* pv_done = p_full + 2;                                   // [2]
   uint64_t* q_full = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
-  int* s_bad = reinterpret_cast<int*>(tmem_slot + 1);   // a draft's V has non-finite elements
+  int* s_bad = reinterpret_cast<int*>(tmem_slot + 1);   // TT_NONFINITE, TT_LOST
   int* s_seq = s_bad + 1;
 
   if (smem - smem_raw > 512) {   // (dynamic shared memory starts 1 KiB aligned)
@@ -468,6 +476,13 @@ __global__ void __launch_bounds__(256, 2)
   const int q_half = L::q_half(act), KS = L::k_stages(act), VS = L::v_stages(act);
   const int off_k = L::HALVES * q_half, off_v = off_k + KS * L::STAGE;
 
+  // (rare; the fence because the barrier before the epilogue orders nothing)
+  auto found = [&](int what) {
+    if (what == TT_LOST) set_status(ERR_BAD_INDEX);
+    atomicOr(s_bad, what);
+    __threadfence_block();
+  };
+
   // ---- loader state (warp 4)
   // TMA: lane i holds the 8-token group of K of chunk i (16 tokens) of eight tiles
   int kid = 0, vid = 0, next = 0;
@@ -476,8 +491,8 @@ __global__ void __launch_bounds__(256, 2)
     if (c * 16 >= s.ctx) return 0;
     int blk = have ? early : table[c * 16 / a.block_size];
     if (blk < 0 || blk >= a.num_blocks) {
-      set_status(ERR_BAD_INDEX);
-      blk = 0;             // load something valid; the result is flagged
+      found(TT_LOST);
+      blk = 0;             // load something valid; nothing of it is stored
     }
     return (blk * 2 * a.n_kv_heads + kvh) * (a.block_size / 8) + c * 16 % a.block_size / 8;
   };
@@ -504,7 +519,7 @@ __global__ void __launch_bounds__(256, 2)
         if (blk >= 0 && blk < a.num_blocks)
           row[h] = ((unsigned)blk * 2 * a.n_kv_heads + kvh) * a.block_size + p % a.block_size;
         else
-          set_status(ERR_BAD_INDEX);
+          found(TT_LOST);
       }
     }
   };
@@ -726,7 +741,7 @@ __global__ void __launch_bounds__(256, 2)
           if (n.x | n.y | n.z | n.w) {
             q.x &= ~n.x, q.y &= ~n.y, q.z &= ~n.z, q.w &= ~n.w;
             *p = q;
-            *s_bad = 1;
+            found(TT_NONFINITE);
           }
         }
         fence_proxy_async_smem();
@@ -790,7 +805,8 @@ __global__ void __launch_bounds__(256, 2)
   else cluster_sync_relaxed();
   const uint32_t to = tmem + L::COL_O + ((uint32_t)((warp & 3) * 32) << 16);
   if (C == 1) {
-    if (warp < act) {
+    const int bad = *s_bad;
+    if (warp < act && !(bad & TT_LOST)) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = a.out + row * a.ld_out + col;
 #pragma unroll
@@ -803,7 +819,7 @@ __global__ void __launch_bounds__(256, 2)
 #pragma unroll
           for (int e = 0; e < 32; e += 8) store_bf16x8(dst + c0 + e, v + e);
       }
-      if (*s_bad != 0 && valid) add_nonfinite<HD>(t, table, kvh, row, s, dst);
+      if (bad && valid) add_nonfinite<HD>(t, table, kvh, row, s, dst);
     }
     tc_fence_before();
     __syncthreads();
@@ -834,16 +850,16 @@ __global__ void __launch_bounds__(256, 2)
             st_cluster_v4(dst + (c0 + e) / 4 * pitch * 16, v[e], v[e + 1], v[e + 2], v[e + 3]);
       }
     }
-    if (*s_bad != 0 && threadIdx.x < C)
-      st_cluster_u32(cluster_map(smem_u32(s_bad), threadIdx.x), 1u);
+    const int mine = *s_bad;
+    if (mine && threadIdx.x < C) red_cluster_or(cluster_map(smem_u32(s_bad), threadIdx.x), mine);
     tc_fence_before();
     cluster_sync_all();          // everything has arrived; nobody touches this CTA's memory after
-    const int r0 = rank * per, n = min(per, nrows - r0);
-    const bool fix = *s_bad != 0;
+    const int bad = *s_bad;
+    const int r0 = rank * per, n = bad & TT_LOST ? 0 : min(per, nrows - r0);
     if (C == 2) merge_rows<HD, 2>(smem, s_ml, s_out + r0, a.out, per, pitch, n);
     else if (C == 4) merge_rows<HD, 4>(smem, s_ml, s_out + r0, a.out, per, pitch, n);
     else merge_rows<HD, 8>(smem, s_ml, s_out + r0, a.out, per, pitch, n);
-    if (fix) {
+    if (bad) {
       __syncthreads();
       for (int i = threadIdx.x; i < n; i += TT_THREADS) {
         const int Ri = rt * TT_ROWS + r0 + i;
