@@ -302,7 +302,8 @@ int tb_argmax(const float* logits, int ld, int M, int N, int* out, void* stream)
  * the same forward writes), parents[row] < i the parent's node index (-1 for
  * the root).  Node i's K/V lie at position ctx_len[s] - q_len[s] + i of the
  * sequence.  Sequences with q_len 0 take part in nothing.  max_q >= every
- * q_len.  Rows of different sequences do not overlap. */
+ * q_len (0 tells the attention that there are no nodes: it launches nothing).
+ * Rows of different sequences do not overlap. */
 
 /* Attention of draft-tree nodes over the paged cache; arguments as
  * tb_paged_attention_decode, bt_w the columns of a block-table row (bt_ld

@@ -339,6 +339,19 @@ def test_tree_attention_leaves_sequences_with_bad_blocks_out(hq, hkv, hd, bs, at
                 assert torch.equal(out[rest], good[rest]) and bool(out[list(lost)].isnan().all())
 
 
+@pytest.mark.parametrize("hd,bs", [(64, 16), (16, 4)])
+def test_tree_attention_max_q_zero(hd, bs):
+    """max_q = 0 is right for a batch without nodes and reported for any other."""
+    c = Case(4, 2, hd, bs, [4, 3], [30, 7], seed=18)
+    d = c.device()
+    out = c.run(d, max_q=0)
+    torch.cuda.synchronize()
+    assert _native.status(clear=True) == BAD_INDEX and bool(out.isnan().all())
+    out = c.run(dict(d, q_len=i32([0, 0])), max_q=0)
+    torch.cuda.synchronize()
+    assert _native.status() == 0 and bool(out.isnan().all())
+
+
 def test_tree_attention_refuses_arguments():
     c = Case(4, 2, 64, 16, [4], [30], seed=16)
     d = c.device()

@@ -225,7 +225,8 @@ def paged_attention_tree(q, out, kv_pool, *, n_q_heads, n_kv_heads, head_dim, bl
     64`` of word ``j // 64``; ``runtime.tree_masks`` builds it).  Rows that
     see nothing get zeros, rows of no sequence are left as they were.
 
-    ``max_q``: the largest ``q_len`` (default: as many as the mask can name).
+    ``max_q``: the largest ``q_len`` (default: as many as the mask can name); a
+    sequence that has more sets the status word and its rows are not written.
     ``max_ctx`` / ``ctx_total``: the longest context and their sum where the
     caller knows them (they only choose how a context is shared out)."""
     lib = N.load()
@@ -244,7 +245,7 @@ def paged_attention_tree(q, out, kv_pool, *, n_q_heads, n_kv_heads, head_dim, bl
             blocks, n_q_heads, n_kv_heads, head_dim, block_size, bp, ldb, width,
             _vec("q_start", q_start, _I32, seqs, dev), _vec("q_len", q_len, _I32, seqs, dev),
             _vec("ctx_len", ctx_len, _I32, seqs, dev), n, mp, ldm, words,
-            min(rows, 64 * words) if max_q is None else max_q, max_ctx, ctx_total)
+            min(rows, 64 * words) if max_q is None else max_q or 1, max_ctx, ctx_total)
 
 
 def _tree(ids, parents, q_start, q_len, n_accepted, path, next_ids, dev):
