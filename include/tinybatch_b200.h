@@ -301,9 +301,9 @@ int tb_argmax(const float* logits, int ld, int M, int N, int* out, void* stream)
  * (i < q_len[s] <= 256), node 0 the root (the last accepted token, whose K/V
  * the same forward writes), parents[row] < i the parent's node index (-1 for
  * the root).  Node i's K/V lie at position ctx_len[s] - q_len[s] + i of the
- * sequence.  Sequences with q_len 0 take part in nothing.  max_q >= every
- * q_len (0 tells the attention that there are no nodes: it launches nothing).
- * Rows of different sequences do not overlap. */
+ * sequence.  Sequences with q_len 0 take part in nothing, whatever their other
+ * metadata.  max_q >= every q_len (0 tells the attention that there are no
+ * nodes: it launches nothing).  Rows of different sequences do not overlap. */
 
 /* Attention of draft-tree nodes over the paged cache; arguments as
  * tb_paged_attention_decode, bt_w the columns of a block-table row (bt_ld

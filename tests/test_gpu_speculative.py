@@ -820,6 +820,29 @@ def test_keep_path_lengths_whose_difference_wraps_move_nothing(ctx):
         assert torch.equal(want, d.cpu())
 
 
+@pytest.mark.parametrize("q_start,ctx", [(-1, -1), (10**6, 10**6), (-2**31, -2**31), (2**31 - 1, 2**31 - 1)])
+def test_sequences_without_nodes_take_part_in_nothing(q_start, ctx):
+    """A padding row of the batch may hold anything beside its q_len of 0."""
+    for hd, bs in ((64, 16), (16, 4)):
+        c = Case(4, 2, hd, bs, [4, 0, 3], [30, 5, 7], seed=19)
+        d = c.device()
+        d["q_start"][1], d["ctx"][1], d["bt"][1] = q_start, ctx, -7
+        c.check(c.run(d, max_q=4))
+    ids, parents, lens, at = i32([0, 1, 2, 0, 1]), i32([-1, 0, 1, -1, 0]), i32([3, 0, 2]), i32([0, q_start, 3])
+    p, u = torch.eye(3, device=DEV)[[1, 2, 0, 1, 2]].contiguous(), torch.full((5,), 0.5, device=DEV)
+    for verify in (lambda *o: ops.verify_drafts(ids, parents, at, lens, p, u, *o),
+                   lambda *o: ops.verify_drafts_greedy(ids, parents, at, lens, i32([1, 2, 0, 1, 2]), *o)):
+        took, path, nxt = outputs(3, 3)
+        verify(took, path, nxt)
+        assert took.tolist() == [2, 0, 1] and nxt.tolist() == [0, -1, 2]
+        assert path.tolist() == [[0, 1, 2], [-1, -1, -1], [0, 1, -1]]
+    dev = [p.to(DEV) for p in random_pools(2, 4, 2, 16, 64)]
+    before = [d.clone() for d in dev]
+    ops.keep_kv_path(dev, block_tables=i32([[0], [99], [1]]), q_len=lens, ctx_len=i32([9, ctx, 9]), path=path,
+                     n_accepted=i32([2, 0, 1]))
+    assert all(torch.equal(a, b) for a, b in zip(dev, before))
+
+
 # ------------------------------------------------------------------ together
 
 

@@ -43,7 +43,8 @@ __device__ __forceinline__ bool tree_seq(const TreeAttnArgs& t, int seq, TreeSeq
   s.ctx = t.a.ctx_len[seq];
   s.base = s.ctx - s.ql;
   // (the lengths compared, not their difference: it may wrap)
-  return s.ql >= 0 && s.ql <= t.max_q && s.ql <= 64 * t.mask_w && s.ctx >= s.ql && s.q0 >= 0 &&
+  if (s.ql == 0) return true;      // takes part in nothing: the rest may be anything
+  return s.ql > 0 && s.ql <= t.max_q && s.ql <= 64 * t.mask_w && s.ctx >= s.ql && s.q0 >= 0 &&
          s.q0 <= t.n_rows - s.ql &&
          s.ctx <= (long long)t.bt_w * t.a.block_size && s.ctx <= (1 << 30);
 }

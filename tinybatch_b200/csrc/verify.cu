@@ -66,9 +66,10 @@ struct VerifyArgs {
   const float* uniforms;
 };
 
-// The rows of sequence `seq` lie inside the batch and its tree is not too large.
+// The rows of a sequence lie inside the batch and its tree is not too large (without
+// nodes its first row may be anything).
 __device__ __forceinline__ bool tree_ok(const TreeArgs& t, int q0, int ql) {
-  return ql >= 0 && ql <= VF_NODES && q0 >= 0 && q0 <= t.n_rows - ql;
+  return ql == 0 || (ql > 0 && ql <= VF_NODES && q0 >= 0 && q0 <= t.n_rows - ql);
 }
 
 // ------------------------------------------------------------------- greedy
