@@ -334,8 +334,9 @@ int tb_paged_attention_tree(const void* q, int ld_q, void* out, int ld_out, int 
  * -1 after them; n_accepted[s] how many drafts that is (without the root);
  * next_ids[s] the token that follows the last of them.  A walk that has
  * filled its path stops there.  q_len 0 gives path -1, n_accepted 0, next -1.
- * Parents that are no earlier node, ids outside the vocabulary and rows
- * outside the batch set TB_STATUS_BAD_INDEX; such nodes are never accepted.
+ * Parents that are no earlier node, ids outside the vocabulary (_greedy, which
+ * is not told it: negative ids) and rows outside the batch set
+ * TB_STATUS_BAD_INDEX; such nodes are never accepted.
  *
  * _greedy: the accepted child is the first whose id is target_ids[row of the
  * node] (the target's argmax there); next is target_ids of the last node.

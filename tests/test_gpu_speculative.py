@@ -587,6 +587,17 @@ def test_verify_bad_trees_are_refused():
         assert status == BAD_INDEX
 
 
+def test_verify_greedy_never_accepts_negative_ids():
+    """A draft without an id does not match a node without a choice."""
+    took, path, nxt = outputs(2, 3)
+    ops.verify_drafts_greedy(i32([-1, -1, 4, -1, 4, 2]), i32([-1, 0, 0, -1, 0, 1]), i32([0, 3]), i32([3, 3]),
+                             i32([-1, 3, 3, 4, 2, 7]), took, path, nxt)
+    torch.cuda.synchronize()
+    assert _native.status(clear=True) == BAD_INDEX
+    assert took.tolist() == [0, 2] and nxt.tolist() == [-1, 7]      # (a root's id is not looked at)
+    assert path.tolist() == [[0, -1, -1], [0, 1, 2]]
+
+
 def test_verify_refuses_arguments():
     ids = i32([0, 1])
     p, u = torch.full((2, 3), 1 / 3, device=DEV), torch.zeros(2, device=DEV)

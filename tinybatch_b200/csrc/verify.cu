@@ -93,12 +93,13 @@ __global__ void __launch_bounds__(VG_WARPS * 32)
   } else if (ql > 0) {
     for (int i = lane; i < ql; i += 32) {
       int p = t.parents[q0 + i];
-      if (i > 0 && (p < 0 || p >= i)) {   // unreachable
+      const int id = t.ids[q0 + i];
+      if (i > 0 && (p < 0 || p >= i || id < 0)) {   // unreachable
         set_status(ERR_BAD_INDEX);
         p = -1;
       }
       s_par[warp][i] = i > 0 ? p : -1;
-      s_id[warp][i] = t.ids[q0 + i];
+      s_id[warp][i] = id;
       s_tgt[warp][i] = target_ids[q0 + i];
     }
     __syncwarp();
