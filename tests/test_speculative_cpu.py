@@ -136,6 +136,27 @@ def test_copy_blocks_checks_its_pairs_on_the_host():
         cache.copy_blocks([(0, 2), (2, 3)])
 
 
+def test_cache_handle_follows_its_pools(monkeypatch):
+    """The handle of the cache moves never keeps the address of storage that a pool
+    has left, whether the tensor or what it holds was exchanged."""
+    monkeypatch.setattr(ops, "_device", lambda t: -1)     # CPU tensors stand for the pools
+    cache = PagedKVCache(3, 4, 16, 1, 64, device="cpu")
+
+    def current():
+        return list(cache.handle().addresses) == [p.data_ptr() for p in cache.pools]
+    first = cache.handle()
+    assert current() and cache.handle() is first
+    old = cache.pools[1].data
+    cache.pools[1].data = torch.ones_like(old)
+    assert current() and cache.handle() is not first
+    cache.pools[2].set_(torch.ones_like(old))
+    assert current()
+    cache.pools[0] = torch.zeros_like(old)
+    assert current()
+    cache.pools = cache.pools[:2]
+    assert current()
+
+
 def test_tree_masks():
     mask, depth = tree_masks([[-1, 0, 0, 1], [-1], []])
     assert mask.dtype == np.int64 and mask.tolist() == [[1], [3], [5], [11], [1]]

@@ -40,7 +40,8 @@ class PagedKVCache:
         """The pools as one argument of ``ops.keep_kv_path`` / ``copy_kv_blocks``."""
         h = self._handle
         if h is None or len(h.pools) != len(self.pools) or any(
-                a is not b for a, b in zip(h.pools, self.pools)):
+                a is not b or b.data_ptr() != p
+                for a, b, p in zip(h.pools, self.pools, h.addresses)):
             h = self._handle = ops.KVPools(self.pools)
         return h
 

@@ -306,7 +306,8 @@ def verify_drafts(ids, parents, q_start, q_len, probs, uniforms, n_accepted, pat
 
 class KVPools:
     """The layers' KV pools as one argument of the cache moves: checked once,
-    their addresses in a host array.  Holds the tensors."""
+    their addresses in a host array.  Holds the tensors; a pool whose storage is
+    exchanged needs a new one."""
 
     def __init__(self, pools):
         """``pools``: a list of ``[num_blocks, 2, n_kv, block_size, head_dim]``
@@ -345,9 +346,9 @@ class KVPools:
             if len(set(ptrs)) != layers:
                 raise ValueError("pools: a layer is listed twice")
         self.pools = pools
-        self._addresses = array("Q", ptrs)      # what the first of args points to
+        self.addresses = array("Q", ptrs)      # what the first of args points to
         # the C calls' first arguments: the addresses, the layers, a pool's shape
-        self.args = (self._addresses.buffer_info()[0], layers, blocks, heads, size, dim)
+        self.args = (self.addresses.buffer_info()[0], layers, blocks, heads, size, dim)
 
 
 def _pools(pools) -> KVPools:
