@@ -235,6 +235,27 @@ def test_forward_tree_refuses_negative_blocks_inside_the_context():
     assert md.slots.tolist() == [63, 32] and md.tree_bt.tolist() == [[3, -1], [0, 2]]
 
 
+def test_buffers_of_growing_batches_are_replaced_a_few_times_only():
+    """Trees that grow a row a step: the retired sets, which stay for graphs over them, hold
+    no more than the one in use."""
+    from types import SimpleNamespace
+
+    from tinybatch_b200.config import named_config
+    from tinybatch_b200.runtime import DeviceModel
+    dm = DeviceModel.__new__(DeviceModel)
+    dm.cfg, dm.device = named_config("tiny"), "cpu"
+    dm.w = SimpleNamespace(n_q=2, ff=dm.cfg.d_ff)
+    dm._alloc(64, 16)
+    for rows in range(1, 600):
+        dm.ensure(rows, rows)
+        assert dm.T_max >= rows and dm.logits.shape[0] >= rows and dm.h.shape[0] == dm.T_max
+    assert dm._alloc_gen == 6                            # 32, 64, 128, 256, 512, 1024 rows of logits
+    retired = sum(t[8].shape[0] for t in dm._retired)
+    assert dm.logits.shape[0] == 1024 and retired <= 1024
+    dm.ensure(5000, 20)
+    assert (dm.T_max, dm.S_max) == (5000, 1024)          # a large batch gets what it needs
+
+
 def test_fork_and_trim_tables():
     bm = BlockManager(8, 4, False)
     table, _ = bm.allocate_prompt(list(range(10)))                # 2 full blocks and half a third

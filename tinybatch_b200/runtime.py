@@ -508,8 +508,11 @@ class DeviceModel:
         self.next_ids = torch.zeros(S, dtype=torch.int32, device=dev)
 
     def ensure(self, T: int, S: int) -> None:
+        # at least doubled, since the old set stays: batches that grow a few rows a step
+        # (draft trees) replace the buffers, and the graphs over them, only a few times
         if T > self.T_max or S > self.S_max:
-            self._alloc(max(T, self.T_max), max(S, self.S_max))
+            self._alloc(max(T, 2 * self.T_max) if T > self.T_max else self.T_max,
+                        max(S, 2 * self.S_max) if S > self.S_max else self.S_max)
 
     # one row-parallel projection: residual (+ all-reduce) + norm prologue
     def _row(self, x, wmat, g_next, T, last: bool, md: StepMeta, site: int, plan):
