@@ -150,6 +150,59 @@ def test_tree_attention_many_words(q_lens, prefix):
     c.check(c.run(c.device()))
 
 
+def shares(c, max_ctx, ctx_total):
+    """(CTAs that share a context, whether sequences start longest first) as the launch
+    chooses them for nodes of one 128-row tile."""
+    n = len(c.ctx)
+    assert max(c.q_lens) * (c.hq // c.hkv) <= 128
+    per = max(ctx_total * c.hkv // 296, 256)
+    split = next(k for k in (8, 4, 2, 1) if max_ctx // per >= k or k == 1)
+    return split, (1 < n <= 64 and split * c.hkv * n > 296 and 4 * max_ctx * n > 5 * ctx_total
+                   and max_ctx // split >= 1024)
+
+
+@pytest.mark.parametrize("hq,hkv,hd,bs", [(10, 2, 128, 16), (7, 1, 64, 32), (5, 1, 128, 8)])
+@pytest.mark.parametrize("split", [1, 2, 8])
+def test_tree_attention_many_tiles_a_cta(hq, hkv, hd, bs, split):
+    """A CTA that walks far more than 16 key tiles: every window of eight tiles' block
+    ids, every lap of the rings."""
+    c = Case(hq, hkv, hd, bs, [9, 1, 5], [1100 * split + 700, 1089, 64 * 33 * split - 5], seed=20 + split)
+    hints = dict(max_ctx=300 * split, ctx_total=300 * split if split == 1 else 300)
+    assert shares(c, **hints)[0] == split and min(c.ctx[0], c.ctx[2]) / split > 17 * 64
+    c.check(c.run(c.device(), max_q=9, **hints))
+
+
+@pytest.mark.parametrize("n,hkv,longest,total,split", [
+    (40, 8, 1100, 33000, 1),            # more sequences than lanes of a warp
+    (64, 8, 1030, 50000, 1), (20, 16, 1500, 22500, 1), (10, 8, 8192, None, 4)])
+@pytest.mark.parametrize("hd,bs", [(64, 16), (64, 8)])
+def test_tree_attention_longest_sequences_first(n, hkv, longest, total, split, hd, bs):
+    """Ragged batches whose CTAs take the sequences by length: ties, a sequence without
+    nodes, and one whose bad length ranks first."""
+    rng = random.Random(n)
+    if total is None:
+        prefix = [rng.choice([3500, 3700, 3700, 4300]) for _ in range(n)]
+    else:
+        prefix = [rng.choice([0, 33, 33, 200, rng.randint(1, 400)]) for _ in range(n)]
+    at, none, bad = n // 2, 2, n - 2
+    q_lens = [rng.randint(1, 3) for _ in range(n)]
+    q_lens[none] = 0
+    prefix[at] = longest - q_lens[at]
+    c = Case(hkv, hkv, hd, bs, q_lens, prefix, seed=21)
+    total = total or sum(c.ctx)
+    assert shares(c, longest, total) == (split, True)
+    d = c.device()
+    good = c.run(d, max_q=3, max_ctx=longest, ctx_total=total)
+    c.check(good)
+    d["ctx"][bad] = 10**9
+    out = c.run(d, max_q=3, max_ctx=longest, ctx_total=total)
+    torch.cuda.synchronize()
+    assert _native.status(clear=True) == BAD_INDEX
+    lost = range(c.q_start[bad], c.q_start[bad] + q_lens[bad])
+    rest = [i for i in range(sum(q_lens)) if i not in lost]
+    assert torch.equal(out[rest], good[rest]) and bool(out[list(lost)].isnan().all())
+
+
 @pytest.mark.parametrize("hints", [dict(), dict(max_ctx=1, ctx_total=1), dict(max_ctx=10**6, ctx_total=5),
                                    dict(max_ctx=5, ctx_total=10**12)])
 def test_tree_attention_hints_only_share_out(hints):
@@ -489,6 +542,44 @@ def test_verify_sampled_wide_and_strided(vocab, pad, shift):
                           path, nxt, draft_probs=place(q), draft_rows=rows.to(DEV))
         assert (took.tolist(), path.tolist(), nxt.tolist()) == R.verify(
             ids, parents, starts(lens), lens, p, u, 8, q, rows)
+
+
+@pytest.mark.parametrize("n,vocab", [
+    (12, 152064), (10, 20011), (80, 152064), (160, 50257), (200, 152064), (300, 20000), (300, 152064),
+    (9, 200003), (2, 163841), (1, 400000)])
+@pytest.mark.parametrize("kind", ["drawn", "picked"])
+def test_verify_sampled_serving_sizes(n, vocab, kind):
+    """Real vocabularies in batches of every cluster size (8, 4, 2 and 1 CTAs a sequence
+    from 10 sequences on): several batches of a segment, several steps of a batch; and few
+    sequences whose vocabulary takes more than one step of 16 CTAs."""
+    rng = random.Random(n + vocab)
+    g = torch.Generator(device=DEV).manual_seed(n + vocab)
+    nodes = 9 if n < 10 else 5 if n < 50 else 3
+    lens = [nodes if i == 0 else rng.randint(0, nodes) for i in range(n)]
+    parents = [p for k in lens for p in (random_tree(rng, k, 3) if k else [])]
+    T = len(parents)
+    p = torch.softmax(torch.randn(T, vocab, generator=g, device=DEV) * 3, -1)
+    # a draft that often misses: siblings are reached, residuals sampled
+    q = 0.6 * torch.softmax(torch.randn(T, vocab, generator=g, device=DEV) * 3, -1) + 0.4 * p
+    parent_row = [a + max(x, 0) for a, k in zip(starts(lens), lens) for x in parents[a:a + k]]
+    taken = {}
+    ids = [0] * T
+    for i, par in enumerate(parents):
+        if par < 0:
+            continue
+        w = q[parent_row[i]].clone()
+        w[taken.get(parent_row[i], [])] = 0
+        ids[i] = int(torch.multinomial(w, 1, generator=g))
+        taken.setdefault(parent_row[i], []).append(ids[i])
+    u = torch.rand(T, generator=g, device=DEV)
+    rows = torch.arange(T, dtype=torch.int32, device=DEV)
+    took, path, nxt = outputs(n, 4)
+    extra = dict(draft_probs=q, draft_rows=rows) if kind == "drawn" else {}
+    ops.verify_drafts(i32(ids), i32(parents), i32(starts(lens)), i32(lens), p, u, took, path, nxt, max_q=nodes,
+                      **extra)
+    drawn = (q.cpu(), rows.cpu()) if kind == "drawn" else (None, None)
+    want = R.verify(ids, parents, starts(lens), lens, p.cpu(), u.cpu(), 4, *drawn)
+    assert (took.tolist(), path.tolist(), nxt.tolist()) == want
 
 
 def test_verify_sampled_corners():

@@ -105,6 +105,20 @@ def test_cache_move_argument_errors(lib):
     assert copy(one, n=0) == 0 and copy(None, layers=0) == 0 and keep(one, n=0) == 0
 
 
+@pytest.mark.parametrize("change,needle", [
+    (dict(blocks=0), "pool shape"), (dict(hkv=0), "pool shape"), (dict(bs=0), "pool shape"), (dict(hd=12), "head_dim"),
+    (dict(layers=-1), "pool shape"), (dict(pools=None), "pools_h"), (dict(pools=P + 8), "aligned"),
+    (dict(pools=0), "aligned"), (dict(n=-1), "n_pairs"), (dict(pairs=None), "pairs"), (dict(pairs=P + 4), "pairs"),
+    (dict(bs=1 << 20, hd=1 << 10), "1 GiB")])
+def test_copy_refusals_name_their_reason(lib, change, needle):
+    a = dict(pools=P, layers=1, blocks=4, hkv=2, bs=16, hd=64, pairs=P, n=1, stream=None)
+    a.update(change)
+    if a["pools"] is not None:
+        a["pools"] = pools_h(a["pools"] or None)
+    assert lib.tb_copy_kv_blocks(*a.values()) == 1
+    assert needle in lib.tb_last_error().decode()
+
+
 def test_cpu_tensors_are_refused():
     with pytest.raises(ValueError, match="CUDA"):
         ops.KVPools(torch.zeros(1, 4, 2, 1, 16, 64, dtype=torch.bfloat16))
