@@ -1057,3 +1057,110 @@ def test_speculative_greedy_decoding_equals_plain_decoding(name):
     for t in tables:
         bm.free_table(t)
     assert bm.num_free() == 64
+
+
+def small_model(name):
+    from tinybatch_b200 import weights
+    from tinybatch_b200.config import named_config
+    from tinybatch_b200.model import Qwen2Paged
+    cfg = named_config("tiny") if name == "tiny" else named_config(
+        "tiny", d_model=512, n_heads=8, n_kv_heads=2, head_dim=64, d_ff=768)
+    return Qwen2Paged.from_weights(cfg, weights.synthetic_weights(cfg, seed=0), DEV)
+
+
+# logits of one token in two batch shapes: two layers of six bf16 roundings (2^-8 each)
+NOISE = 2 * 6 * 2**-8
+
+
+def plain_logits(model, tokens, bs=16):
+    """Logits after ``tokens`` from a prefill of all of them in a cache of its own."""
+    blocks = -(-len(tokens) // bs)
+    return model.forward(tokens, list(range(len(tokens))), [(0, len(tokens))], [list(range(blocks))], [len(tokens)],
+                         model.make_kv_cache(blocks, bs))[0]
+
+
+@pytest.mark.parametrize("name", ["tiny", "mid"])
+def test_forward_tree_equals_the_plain_forward(name):
+    """Every node's logits are those of a causal forward over the prompt and the
+    node's path: positions, masks and slots, for branches, chains and a lone root."""
+    model = small_model(name)
+    V, bs = model.cfg.vocab_size, 16
+    rng = random.Random(1)
+    prompts = [[rng.randrange(V) for _ in range(k)] for k in (37, 16, 1, 90)]
+    parents = [random_tree(rng, 12, 3), [-1] + list(range(6)), [-1, 0, 0, 0], [-1]]
+    ids = [[rng.randrange(V) for _ in par] for par in parents]
+    ctx = [len(p) + len(t) for p, t in zip(prompts, parents)]
+    need = [-(-c // bs) for c in ctx]
+    order = list(range(sum(need)))
+    rng.shuffle(order)
+    tables = [order[a:a + k] for a, k in zip(starts(need), need)]
+    cache = model.make_kv_cache(sum(need), bs)
+    ends = np.cumsum([len(p) for p in prompts]).tolist()
+    model.forward([t for p in prompts for t in p], [i for p in prompts for i in range(len(p))],
+                  [(e - len(p), e) for e, p in zip(ends, prompts)], tables, [len(p) for p in prompts], cache)
+    _, logits = model.forward_tree([t for n in ids for t in n], parents, tables, ctx, cache)
+    logits, r0 = logits.clone(), 0
+    for prompt, par, node_ids in zip(prompts, parents, ids):
+        for i in range(len(par)):
+            path, j = [], i
+            while j >= 0:
+                path.append(node_ids[j])
+                j = par[j]
+            want = plain_logits(model, prompt + path[::-1])
+            assert float((logits[r0 + i] - want).abs().max()) <= NOISE * float(want.abs().max()), (r0, i)
+        r0 += len(par)
+
+
+def test_accepted_drafts_in_the_prefix_cache_hold_their_keys_and_values():
+    """Steps of drafts in room from BlockManager.reserve, trimmed and published with the
+    prefix cache on: a later prompt that finds the blocks computes only its tail,
+    and its logits are those of a prefill of everything."""
+    from tinybatch_b200.block_manager import BlockManager
+    model = small_model("tiny")
+    V, bs = model.cfg.vocab_size, 16
+    rng = random.Random(2)
+    bm, cache = BlockManager(64, bs), model.make_kv_cache(64, bs)
+    seqs = [[rng.randrange(V) for _ in range(k)] for k in (20, 5)]
+    tables = [bm.allocate_prompt(s)[0] for s in seqs]
+    ends = np.cumsum([len(s) for s in seqs]).tolist()
+    logits = model.forward([t for s in seqs for t in s], [i for s in seqs for i in range(len(s))],
+                           [(e - len(s), e) for e, s in zip(ends, seqs)], tables, [len(s) for s in seqs], cache)
+    for s, t in zip(seqs, logits.argmax(-1).tolist()):
+        s.append(t)
+    moved = 0
+    for step in range(12):
+        ids, parents = [], []
+        for s in seqs:
+            # right tokens (from a plain forward) in a chain, each behind a wrong sibling
+            node_ids, par, at, ahead = [s[-1]], [-1], 0, list(s)
+            for k in range(rng.randint(1, 4)):
+                right = int(plain_logits(model, ahead).argmax())
+                ahead.append(right)
+                node_ids += [(right + 1) % V, right if rng.random() < 0.9 else (right + 2) % V]
+                par += [at, at]
+                at = len(par) - 1
+            ids.append(node_ids)
+            parents.append(par)
+        ctx = [len(s) - 1 + len(n) for s, n in zip(seqs, ids)]
+        for t, c in zip(tables, ctx):
+            bm.reserve(t, c)
+        md, target = model.forward_tree([t for n in ids for t in n], parents, tables, ctx, cache, sample=True)
+        took, path, nxt = outputs(2, 6)
+        ops.verify_drafts_greedy(md.ids, i32([p for t in parents for p in t]), md.tree_q_start, md.tree_q_len, target,
+                                 took, path, nxt, max_q=md.tree_max_q)
+        cache.keep_path(block_tables=md.tree_bt, q_len=md.tree_q_len, ctx_len=md.tree_ctx, path=path, n_accepted=took)
+        for s, t, node_ids, a, pth, nx in zip(seqs, tables, ids, took.tolist(), path.tolist(), nxt.tolist()):
+            before = len(s)
+            s += [node_ids[j] for j in pth[1:a + 1]] + [nx]
+            moved += a
+            bm.trim_table(t, len(s) - 1)
+            bm.publish(t, s[:-1], before - 1)
+    assert moved > 12
+    for s, t in zip(seqs, tables):
+        prompt = s + [7, 8, 9]
+        table, cached = bm.allocate_prompt(prompt)
+        assert cached == (len(s) - 1) // bs * bs >= bs and table[:cached // bs] == t[:cached // bs]
+        got = model.forward(prompt[cached:], list(range(cached, len(prompt))), [(0, len(prompt) - cached)], [table],
+                            [len(prompt)], cache)[0]
+        want = plain_logits(model, prompt)
+        assert float((got - want).abs().max()) <= NOISE * float(want.abs().max())
