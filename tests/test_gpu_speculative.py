@@ -1098,14 +1098,16 @@ def test_forward_tree_equals_the_plain_forward(name):
     ends = np.cumsum([len(p) for p in prompts]).tolist()
     model.forward([t for p in prompts for t in p], [i for p in prompts for i in range(len(p))],
                   [(e - len(p), e) for e, p in zip(ends, prompts)], tables, [len(p) for p in prompts], cache)
-    _, logits = model.forward_tree([t for n in ids for t in n], parents, tables, ctx, cache)
-    logits, r0 = logits.clone(), 0
+    md, logits = model.forward_tree([t for n in ids for t in n], parents, tables, ctx, cache)
+    logits, positions, r0 = logits.clone(), md.positions.tolist(), 0
     for prompt, par, node_ids in zip(prompts, parents, ids):
         for i in range(len(par)):
             path, j = [], i
             while j >= 0:
                 path.append(node_ids[j])
                 j = par[j]
+            # (a rotary position off by one would move the logits by less than the tolerance)
+            assert positions[r0 + i] == len(prompt) + len(path) - 1
             want = plain_logits(model, prompt + path[::-1])
             assert float((logits[r0 + i] - want).abs().max()) <= NOISE * float(want.abs().max()), (r0, i)
         r0 += len(par)
