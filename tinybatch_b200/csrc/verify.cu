@@ -93,14 +93,14 @@ __global__ void __launch_bounds__(VG_WARPS * 32)
   } else if (ql > 0) {
     for (int i = lane; i < ql; i += 32) {
       int p = t.parents[q0 + i];
-      const int id = t.ids[q0 + i];
+      const int id = t.ids[q0 + i], tgt = target_ids[q0 + i];   // (all loads before the checks)
       if (i > 0 && (p < 0 || p >= i || id < 0)) {   // unreachable
         set_status(ERR_BAD_INDEX);
         p = -1;
       }
       s_par[warp][i] = i > 0 ? p : -1;
       s_id[warp][i] = id;
-      s_tgt[warp][i] = target_ids[q0 + i];
+      s_tgt[warp][i] = tgt;
     }
     __syncwarp();
     int c = 0;
