@@ -11,11 +11,13 @@
 // written once.  Measured on a B200 (CUDA graph, inputs rotated through more than
 // the L2): 200 blocks of 64 KiB in 48 layers 147 us (629 MB written, 0.27 GB of
 // distinct sources read: 6.1 TB/s, 0.94 of the copy bandwidth); the accepted paths of
-// 64 sequences, 162 tokens in 48 layers, 16 us: 65 MB in runs of 256 bytes, all that
-// a pool keeps contiguous of a token and head, 4.0 TB/s.  More loads in flight a
-// thread, one wave of CTAs over several layers each, or fewer dependent loads before
-// the moves did not change the latter: the runs' scatter over DRAM pages bounds it.
-// Paths that are in place (chains) return before the pools: 7.1 us.  Leaving out the
+// 64 sequences, 162 tokens in 48 layers, 15.9 us: 65 MB in runs of 256 bytes, all that
+// a pool keeps contiguous of a token and head, 4.1 TB/s.  Paths that are in place (chains)
+// return before the pools after 6.8 us: the start of 3072 CTAs, each with its loads of
+// lengths, path and block ids that wait for one another.  So much of the 15.9 us passes
+// without a move, and the moves take what the floor allows them (9.7 us); DRAM is a
+// quarter busy.  More loads in flight a thread, one wave of CTAs over several layers each,
+// or fewer dependent loads before the moves did not change the total.  Leaving out the
 // nodes in front of a path that moves costs the others more (a loop from a start of
 // their own: 20.7 instead of 16.0 us) than it saves.
 #include "common.cuh"

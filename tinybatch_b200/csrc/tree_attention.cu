@@ -172,29 +172,34 @@ static int tree_simple_launch(const TreeAttnArgs& t, cudaStream_t st) {
 //              128-byte swizzle: K is a K-major operand and V an MN-major one.  Four
 //              lanes issue a tile's boxes.  Other block sizes: 16-byte cp.async
 //              pieces into the same layout, every key looking up its block (1.25 to 2
-//              times as long: blocks of 8 take 10 / 88 / 69 / 323 us where blocks of
-//              16 take 8 / 58 / 48 / 161 on the cases below, the lone one first).  K
+//              times as long: blocks of 8 take 10 / 89 / 69 / 322 us where blocks of
+//              16 take 8 / 59 / 48 / 158 on the cases below, the lone one first).  K
 //              and V have rings of their own: a K stage is free once its S is done,
 //              before the V that came with it
 //   warp 5     MMA issue.  P (bf16) has two buffers of its own in TMEM, so S of the
 //              next tile follows as soon as the softmax has S in registers and is
 //              there when it has written P
+// P is rounded to bf16 because the MMA takes bf16 for both operands, as in the decode
+// and prefill kernels; its sum is taken of the unrounded weights, in fp32.  The output's
+// error against 64 bits is 0.0021-0.0023 relative where rounding the output alone
+// gives 0.0017; a second MMA with P's rest would half again lengthen the MMA work.
 // O is accumulated in TMEM; a row's exponent reference moves only when its
 // maximum has grown by more than TT_RESCALE (log2 units), as in the prefill kernel.
 // Two CTAs an SM: one's chain S -> softmax -> P V, its start and its end hide
 // behind the other's loads.
 //
 // Measured on a B200 (CUDA graph, inputs rotated through more than the L2): 32
-// chains of 6 drafts over 500-4000 tokens (40/8 heads of 128) 57.5 us, 5.3 TB/s or
-// 0.81 of the measured copy bandwidth; 16 trees of 25 over 300-6000 tokens 48.4 us,
+// chains of 6 drafts over 500-4000 tokens (40/8 heads of 128) 58.7 us, 5.2 TB/s or
+// 0.80 of the measured copy bandwidth; 16 trees of 25 over 300-6000 tokens 48.4 us,
 // 0.61 of it (what is missing: ~2.5 us before a CTA's first tile, 4-5 us of merge over
 // the cluster with the wait for its members, the tail of the ragged batch); 4 trees of
-// 64 over 12-20 thousand tokens, 512 rows a kv head, 154-162 us from board to board,
-// 880-835 TFLOP/s or 0.54-0.51 of the measured bf16 peak: there the softmax's chain of
+// 64 over 12-20 thousand tokens, 512 rows a kv head, 155-158 us in a burst, 873-857
+// TFLOP/s or 0.53-0.52 of the measured bf16 peak (182 us, 744 TFLOP/s or 0.55 of the
+// sustained peak, where seconds of it bring the power cap and 1.66 GHz): there the softmax's chain of
 // dependent instructions bounds it (tensor pipe 52% busy, exponentials 49%).  A lone
-// short request takes 7.7-8.0 us: launch, lengths, block ids, K, S, softmax, P V and
-// the store one after another.  At the 128 registers a thread 11 words spill at
-// head_dim 128 (8 at 64); with more registers a CTA waits for an empty SM.
+// short request takes 7.5-7.9 us: launch, lengths, block ids, K, S, softmax, P V and
+// the store one after another.  At the 128 registers a thread 10 words spill at
+// head_dim 128 (7 at 64); with more registers a CTA waits for an empty SM.
 // Tried and dropped: 16-byte cp.async for all loads (one warp issues 9 B a cycle: 94
 // instead of 64 us for the trees), two threads a row (the exchange of maxima costs what
 // the shorter softmax saves), K and V boxes issued together (K waits for V's stage).
@@ -899,10 +904,11 @@ static int tree_pool_map(CUtensorMap* map, const AttnArgs& a) {
   return TB_OK;
 }
 
-// CTAs that share a context: as many as let the longest context's share be no
-// longer than the average work of a resident CTA (148 SMs x 2), so that one wave covers a
-// small batch and a long context does not outlast the others, but no share
-// below four tiles (the merge costs more than it saves).
+// CTAs that share a context: the power of two, at most 8, that brings the longest
+// context's share down to once to twice the average work of a resident CTA (148 SMs x 2;
+// more where 8 are too few), so that one wave covers a small batch and a long context
+// does not outlast the others by much, but no share below four tiles (the merge
+// costs more than it saves).
 static int tree_splits(int n_seqs, int n_kv, int row_tiles, int max_ctx, long long ctx_total) {
   const long long share = ctx_total * n_kv * row_tiles / (148 * 2);
   const long long least = 4 * TT_KEYS;
@@ -926,7 +932,10 @@ static int tree_tc_launch(TreeAttnArgs t, int max_ctx, long long ctx_total, cuda
   const int C = tree_splits(t.a.n_seqs, t.a.n_kv_heads, row_tiles, max_ctx, ctx_total);
   t.log_splits = C == 8 ? 3 : C == 4 ? 2 : C - 1;
   // More CTAs than fit at once and ragged, long contexts: longest sequences first,
-  // so that none starts late (ranking them costs ~0.5 us a CTA)
+  // so that none starts late (ranking them costs ~0.5 us a CTA).  Device us without / with:
+  // 32 chains over 500-4000 tokens 60.4 / 58.8, 16 trees over 300-6000 55.9 / 48.3, 64
+  // chains over 100-4000 106 / 89; lengths within a third of one another, left in the
+  // caller's order, 82.4 / 83.8
   const int n = t.a.n_seqs;
   t.by_length = n > 1 && n <= 64 && (long long)C * t.a.n_kv_heads * row_tiles * n > 148 * 2 &&
                 4ll * max_ctx * n > 5 * ctx_total && max_ctx / C >= 1024;

@@ -27,10 +27,10 @@
 // move with the summation order in 32.
 //
 // What bounds them (B200, CUDA graph, vocabulary 152064).  Greedy: launch and two
-// dependent loads, 2.4 us for one sequence, 3.3 us for 128.  Sampled: steps that wait
-// for one another.  One sequence, outright drafts 8.8 us; stamps of an instrumented
+// dependent loads, 2.3 us for one sequence, 3.3 us for 128.  Sampled: steps that wait
+// for one another.  One sequence, outright drafts 9.0 us; stamps of an instrumented
 // build: loads of rows, tree and probabilities 2.1 us, walk 1.7, pass over the last
-// node's rows 1.9, sums over the cluster 1.4, search 2.4.  64 chains 26.5 us, of them
+// node's rows 1.9, sums over the cluster 1.4, search 2.4.  64 chains 26.6 us, of them
 // ~14 in the pass (78 MB, the floor of the call is 11.9 us).  8 trees of 40 nodes
 // 23.3 us: the slowest walk takes 13, as each Z is a pass that decides the next
 // sibling's test; the floor counts one pass.
@@ -619,8 +619,14 @@ int verify_launch(const VerifyArgs& a, int max_q, cudaStream_t st) {
     return arg_err("draft_probs and draft_rows go together");
   if (a.draft_probs != nullptr && (a.ld_d < a.vocab || a.n_draft_rows < 0))
     return arg_err("draft_probs shape");
-  // few sequences: clusters of 16 (a sequence on 16 SMs); many: smaller CTAs, four an SM, in
-  // one wave
+  // few sequences: clusters of 16 (a sequence on 16 SMs, r kept between the passes at a
+  // node); many: smaller CTAs, four an SM, in one wave.  Device us of either form at a vocabulary of
+  // 152064, first / second: 8 sequences: chains of 6 16.2 / 17.0, trees of 40 23.4 / 65.7,
+  // outright trees of 26 15.2 / 15.8; 12: 17.4 / 17.4, 30.5 / 66.8, 16.8 / 15.2; 16:
+  // 24.2 / 18.4, 34.4 / 67.4, 23.0 / 15.7; 48: 61.9 / 25.5, 104 / 91, 58.6 / 21.0.  The
+  // border is where the first form's CTAs stop fitting at once, which suits chains; trees
+  // with siblings to reject would gain from it up to about 32 sequences, but what a batch
+  // holds is not known to the host
   const int n = a.t.n_seqs;
   if (n > 0x7fffffff / VF_MAX_CLUSTER) return arg_err("n_seqs");
   if (n * 16 <= 148) {
