@@ -181,7 +181,7 @@ static int tree_simple_launch(const TreeAttnArgs& t, cudaStream_t st) {
 //              there when it has written P
 // P is rounded to bf16 because the MMA takes bf16 for both operands, as in the decode
 // and prefill kernels; its sum is taken of the unrounded weights, in fp32.  The output's
-// error against 64 bits is 0.0021-0.0023 relative where rounding the output alone
+// error against 64 bits is 0.0021-0.0025 relative where rounding the output alone
 // gives 0.0017; a second MMA with P's rest would half again lengthen the MMA work.
 // O is accumulated in TMEM; a row's exponent reference moves only when its
 // maximum has grown by more than TT_RESCALE (log2 units), as in the prefill kernel.
